@@ -16,7 +16,7 @@ try:
                            fmha_fwd_splitkv_combine, fmha_fwd_varlen, fmha_last_kernel, fmha_num_splits_heuristic, fmha_version)
 except ImportError as e:  # no fallback: say how to build
     raise ImportError(f"the compiled module flash_ck.flash_ck is missing or does not load ({e}); build it with "
-                      f"`python -m flash_ck.build` in {_os.path.dirname(_os.path.dirname(_os.path.abspath(__file__)))}") from e
+                      f"`python flash_ck/build.py` in {_os.path.dirname(_os.path.dirname(_os.path.abspath(__file__)))}") from e
 
 from . import nn, ops  # noqa: E402,F401
 from .nn import Attention, PagedAttention  # noqa: E402,F401

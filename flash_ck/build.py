@@ -1,5 +1,5 @@
 """In-tree build of the compiled module flash_ck/flash_ck<ext>.so (pybind11 + torch tensors over the C ABI of
-flashck_amd/libflashck_fmha.so).  ``python -m flash_ck.build``; needs hipcc, builds without a GPU."""
+flashck_amd/libflashck_fmha.so).  ``python flash_ck/build.py``; needs hipcc, builds without a GPU."""
 import os
 import subprocess
 import sys
