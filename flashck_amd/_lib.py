@@ -18,7 +18,8 @@ class Attrs(ctypes.Structure):
                 ("bias_batch_stride", ctypes.c_int64), ("bias_head_stride", ctypes.c_int64), ("bias_row_stride", ctypes.c_int64),
                 ("logits_soft_cap", ctypes.c_float), ("kv_dtype", ctypes.c_int32), ("k_descale", ctypes.c_float),
                 ("v_descale", ctypes.c_float), ("decode_variant", ctypes.c_int32), ("prefill_variant", ctypes.c_int32),
-                ("bias_cols", ctypes.c_int64), ("max_seqlen_k", ctypes.c_int64), ("o_scale", ctypes.c_float)]
+                ("bias_cols", ctypes.c_int64), ("max_seqlen_k", ctypes.c_int64), ("o_scale", ctypes.c_float),
+                ("lse", ctypes.c_void_p), ("lse_head_stride", ctypes.c_int64)]
 
 
 _ap = ctypes.POINTER(Attrs)
@@ -38,6 +39,11 @@ SIGNATURES = {
     "fck_fmha_fused_reset": (ctypes.c_int, [_vp]),
     "fck_fmha_validate_paged": (ctypes.c_int, [_vp] * 6 + [_i64] * 3 + [_vp, _vp]),
     "fck_fmha_fwd_splitkv_combine": (ctypes.c_int, [_vp] * 4 + [_i64] * 6 + [_i32, _vp]),
+    "fck_fmha_fwd_splitkv_combine_lse": (ctypes.c_int, [_vp] * 5 + [_i64] * 6 + [_i32, _vp]),
+    "fck_fmha_decode_shared_prefix": (ctypes.c_int, [_vp] * 12 + [_i64] * 13 + [_f32, _i64, _i64, _u32, _i32, _ap, _vp]),
+    "fck_fmha_shared_prefix_splits": (ctypes.c_int, [_i64] * 9 + [_vp] * 2),
+    "fck_fmha_key_weights": (ctypes.c_int, [_vp] * 8 + [_i64] * 10 + [_f32, _i64, _i64, _u32, _i32, _ap, _vp]),
+    "fck_fmha_cache_evict": (ctypes.c_int, [_vp] * 10 + [_i64] * 2 + [_vp] + [_i64] * 10 + [_i32, _vp]),
     "fck_fmha_fwd_appendkv": (ctypes.c_int, [_vp] * 7 + [_i64, _vp, _vp, _i64, _i32, _i32, _vp, _i64, _i64, _vp]
                               + [_i64] * 6 + [_i32, _vp]),
     "fck_fmha_fwd_appendkv_attrs": (ctypes.c_int, [_vp] * 7 + [_i64, _vp, _vp, _i64, _i32, _i32, _vp, _i64, _i64, _vp]

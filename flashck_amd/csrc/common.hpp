@@ -222,6 +222,16 @@ __device__ __forceinline__ f32x4_t combine_splits(const float* lse_acc, const fl
     return f32x4_t{acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
 }
 
+// Log-sum-exp over a row's splits, as combine_splits weighs them; -inf when all of them are empty (or there is none).
+__device__ __forceinline__ float combine_lse(const float* lse_acc, int64_t w0, int64_t step, int ns)
+{
+    float m = -INFINITY, sum = 0.f;
+    for (int s = 0; s < ns; ++s) m = fmaxf(m, lse_acc[w0 + s * step]);
+    if (m == -INFINITY) return -INFINITY;
+    for (int s = 0; s < ns; ++s) sum += __expf(lse_acc[w0 + s * step] - m);
+    return m + fast_log2(sum) * kLn2;
+}
+
 // Visible key range [lo, hi) of query row i: GenericAttentionMask::IsOutOfBound,
 // ck_tile/ops/fmha/block/block_masking.hpp:359-373 with (y, x) from
 // make_generic_attention_mask_coordinates_from_lr_window, same file :608-628.

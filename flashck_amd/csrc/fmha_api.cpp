@@ -6,6 +6,7 @@
 
 #include <climits>
 #include <cmath>
+#include <cstddef>
 #include <cstdlib>
 #include <cstdarg>
 #include <cstdio>
@@ -127,6 +128,57 @@ int fill_variant(fck::PrefillArgs& a, const fck_fmha_attrs* at)
     return FCK_OK;
 }
 
+// fck_fmha_attrs without its last fields (lse, lse_head_stride): what callers built against the earlier struct pass
+constexpr size_t kAttrsSizeNoLse = offsetof(fck_fmha_attrs, lse);
+
+int check_attrs_size(const fck_fmha_attrs* at)
+{
+    if (at->size != sizeof(fck_fmha_attrs) && at->size != kAttrsSizeNoLse)
+        return fail(FCK_ERR_INVALID_ARGUMENT, "fck_fmha_attrs.size is %u, this library's struct has %zu bytes", at->size, sizeof(fck_fmha_attrs));
+    return FCK_OK;
+}
+
+bool wants_lse(const fck_fmha_attrs* at) { return at && at->size == sizeof(fck_fmha_attrs) && at->lse; }
+
+// fck_fmha_attrs of an operator that has no kernel variants, no output scale and an lse argument of its own (after fill_mod)
+int only_score_attrs(const fck_fmha_attrs* at)
+{
+    if (!at) return FCK_OK;
+    if (at->decode_variant != 0 || at->prefill_variant != 0 || (at->o_scale != 0.f && at->o_scale != 1.f))
+        return fail(FCK_ERR_INVALID_ARGUMENT, "decode_variant, prefill_variant and o_scale do not apply to this operator");
+    if (wants_lse(at)) return fail(FCK_ERR_INVALID_ARGUMENT, "lse is an argument of this operator: fck_fmha_attrs.lse must be null");
+    return FCK_OK;
+}
+
+// e4m3 cache under 16-bit queries: the K scale multiplies every score, the V scale (v_descale, null: no V) the output
+int fill_cache_type(int32_t& kv8, float& scale_log2, fck::ScoreMod& mod, float* v_descale, const fck_fmha_attrs* at, int64_t d, int64_t dv)
+{
+    kv8 = 0;
+    if (!at || at->kv_dtype == 0) return FCK_OK;
+    if (at->kv_dtype != FCK_DTYPE_FP8) return fail(FCK_ERR_UNSUPPORTED, "kv_dtype %d: only 0 (same as q) and FLOAT8 (1)", at->kv_dtype);
+    const float kd = at->k_descale == 0.f ? 1.f : at->k_descale, vd = at->v_descale == 0.f ? 1.f : at->v_descale;
+    if (!(kd > 0.f) || !std::isfinite(kd) || !(vd > 0.f) || !std::isfinite(vd))
+        return fail(FCK_ERR_INVALID_ARGUMENT, "k_descale and v_descale must be positive and finite (0: 1)");
+    if (d != dv || d != kernel_dim(d, dv)) return fail(FCK_ERR_UNSUPPORTED, "an fp8 K/V cache needs qk_head_dim = v_head_dim in {64, 128, 256}");
+    kv8 = 1;
+    scale_log2 *= kd;
+    mod.scale *= kd;
+    if (v_descale) *v_descale = vd;
+    return FCK_OK;
+}
+
+// log-sum-exp output of a prefill-family call (after fill_mod, which checks the struct's size)
+int fill_lse(fck::PrefillArgs& a, const fck_fmha_attrs* at, int64_t seqlen_q)
+{
+    if (!wants_lse(at)) return FCK_OK;
+    if (reinterpret_cast<uintptr_t>(at->lse) & 3u) return fail(FCK_ERR_INVALID_ARGUMENT, "lse is fp32: the pointer must be 4-byte aligned");
+    if (at->lse_head_stride < (a.seqstart_q ? 1 : seqlen_q))
+        return fail(FCK_ERR_INVALID_ARGUMENT, "lse_head_stride %ld is smaller than a head's row of query tokens", (long)at->lse_head_stride);
+    a.lse = at->lse;
+    a.lse_head_stride = at->lse_head_stride;
+    return FCK_OK;
+}
+
 // Bias / ALiBi / soft cap of a call: `bias` is the positional pointer of the entry points that have one (else null).
 
 int fill_mod(fck::ScoreMod& m, const void* bias, const fck_fmha_attrs* at, float scale, uint32_t mask_type, int64_t hq)
@@ -137,8 +189,7 @@ int fill_mod(fck::ScoreMod& m, const void* bias, const fck_fmha_attrs* at, float
         if (bias) return fail(FCK_ERR_UNSUPPORTED, "a bias pointer needs the _attrs entry point: fck_fmha_attrs says what it holds");
         return FCK_OK;
     }
-    if (at->size != sizeof(fck_fmha_attrs))
-        return fail(FCK_ERR_INVALID_ARGUMENT, "fck_fmha_attrs.size is %u, this library's struct has %zu bytes", at->size, sizeof(fck_fmha_attrs));
+    if (int rc = check_attrs_size(at)) return rc;
     if (!bias) bias = at->bias;
     if (at->bias && bias != at->bias) return fail(FCK_ERR_INVALID_ARGUMENT, "two different bias pointers (argument and fck_fmha_attrs.bias)");
     if (!(at->logits_soft_cap >= 0.f) || !std::isfinite(at->logits_soft_cap))
@@ -317,6 +368,7 @@ static int splitkv_setup(fck::SplitKvArgs& a, bool& uniform, int& rows_max, cons
     a.window_left = window_left;
     a.window_right = window_right;
     if (int rc = fill_mod(a.mod, bias, attrs, scale, mask_type, hq)) return rc;
+    if (wants_lse(attrs)) return fail(FCK_ERR_INVALID_ARGUMENT, "split-KV returns lse_acc; the combine (fck_fmha_fwd_splitkv_combine_lse) merges it");
     a.v_descale = 1.f;
     if (attrs && attrs->decode_variant != 0) {
         const int32_t dvar = attrs->decode_variant;
@@ -520,6 +572,13 @@ int fck_fmha_fwd_splitkv_combine(const void* lse_acc, const void* o_acc, void* o
                                  int64_t seqlen_q, int64_t hq, int64_t dv, int64_t q_max_seq_len, int64_t num_splits,
                                  int32_t dtype, void* stream)
 {
+    return fck_fmha_fwd_splitkv_combine_lse(lse_acc, o_acc, o, nullptr, seqstart_q, batch, seqlen_q, hq, dv, q_max_seq_len, num_splits, dtype, stream);
+}
+
+int fck_fmha_fwd_splitkv_combine_lse(const void* lse_acc, const void* o_acc, void* o, void* lse, const int32_t* seqstart_q, int64_t batch,
+                                     int64_t seqlen_q, int64_t hq, int64_t dv, int64_t q_max_seq_len, int64_t num_splits,
+                                     int32_t dtype, void* stream)
+{
     g_err[0] = 0;
     (void)q_max_seq_len;
     if (dtype != FCK_DTYPE_FP16 && dtype != FCK_DTYPE_BF16 && dtype != FCK_DTYPE_FP8)
@@ -541,6 +600,7 @@ int fck_fmha_fwd_splitkv_combine(const void* lse_acc, const void* o_acc, void* o
     a.dv = (int32_t)dv;
     a.num_splits = (int32_t)num_splits;
     a.num_cu = cu_count();
+    a.lse = static_cast<float*>(lse);
     a.o_scale = 1.f;  // e4m3 output: the reference's wrapper has no scale argument either (fmha_fwd_split_kv_combine_jinja.h:78-92)
     return launch_status(fck::launch_splitkv_combine(a, dtype, static_cast<hipStream_t>(stream)), "FmhaFwdSplitKVCombine launch");
 }
@@ -568,8 +628,8 @@ int fck_fmha_fwd_appendkv_attrs(void* q, void* k_cache, void* v_cache, const voi
     float k_descale = 1.f, v_descale = 1.f;
     int32_t kv8 = 0;
     if (attrs) {
-        if (attrs->size != sizeof(fck_fmha_attrs))
-            return fail(FCK_ERR_INVALID_ARGUMENT, "fck_fmha_attrs.size is %u, this library's struct has %zu bytes", attrs->size, sizeof(fck_fmha_attrs));
+        if (int rc = check_attrs_size(attrs)) return rc;
+        if (wants_lse(attrs)) return fail(FCK_ERR_INVALID_ARGUMENT, "appendKV has no log-sum-exp: fck_fmha_attrs.lse must be null");
         if (attrs->bias_type != 0 || attrs->bias || attrs->logits_soft_cap != 0.f)
             return fail(FCK_ERR_INVALID_ARGUMENT, "appendKV takes no bias / soft cap: only kv_dtype, k_descale and v_descale of fck_fmha_attrs apply");
         if (attrs->kv_dtype != 0) {
@@ -744,6 +804,7 @@ int fck_fmha_fwd_attrs(const void* q, const void* k, const void* v, const void* 
     if (int rc = fill_mod(a.mod, bias, attrs, scale, mask_type, hq)) return rc;
     if (int rc = fill_kv8(a, attrs, d, dv, dtype)) return rc;
     if (int rc = fill_variant(a, attrs)) return rc;
+    if (int rc = fill_lse(a, attrs, seqlen_q)) return rc;
     a.kv.page_shift = -1;
     a.kv.seqlen_k_ptr = seqlen_k_ptr;  // group mode: logical key counts of padded packed sequences
     if (seqstart_q) {
@@ -800,6 +861,7 @@ int fck_fmha_batch_prefill_attrs(const void* q, const void* k_cache, const void*
     if (int rc = fill_mod(a.mod, nullptr, attrs, scale, mask_type, hq)) return rc;
     if (int rc = fill_kv8(a, attrs, d, dv, dtype)) return rc;
     if (int rc = fill_variant(a, attrs)) return rc;
+    if (int rc = fill_lse(a, attrs, 0)) return rc;
     a.kv.mode = 3;
     a.kv.kv_indptr = kv_indptr;
     a.kv.kv_page_indices = kv_page_indices;
@@ -855,6 +917,7 @@ int fck_fmha_fwd_pagedkv_attrs(const void* q, const void* k_cache, const void* v
     if (int rc = fill_mod(a.mod, nullptr, attrs, scale, mask_type, hq)) return rc;
     if (int rc = fill_kv8(a, attrs, d, dv, dtype)) return rc;
     if (int rc = fill_variant(a, attrs)) return rc;
+    if (int rc = fill_lse(a, attrs, seqlen_q)) return rc;
     a.kv.mode = 2;
     a.kv.block_table = block_table;
     a.kv.block_table_stride = (int32_t)batch_stride_block_table;
@@ -863,6 +926,212 @@ int fck_fmha_fwd_pagedkv_attrs(const void* q, const void* k_cache, const void* v
     a.kv.page_shift = log2_exact(page_block_size);
     if (q_max_seq_len <= 0) q_max_seq_len = seqlen_q;
     return prefill_common(a, d, dv, dtype, q_max_seq_len, page_block_size % 64 == 0, stream, "FmhaFwdPagedKV launch");
+}
+
+int fck_fmha_shared_prefix_splits(int64_t batch, int64_t num_groups, int64_t max_group_size, int64_t hq, int64_t hk, int64_t sq,
+                                  int64_t max_prefix_len, int64_t max_own_len, int64_t num_cu, int32_t* prefix_splits, int32_t* own_splits)
+{
+    if (prefix_splits) *prefix_splits = 1;
+    if (own_splits) *own_splits = 1;
+    constexpr int64_t kMax = (int64_t)1 << 24;
+    for (int64_t v : {batch, num_groups, max_group_size, hq, hk, sq})
+        if (v <= 0 || v > kMax) return FCK_OK;
+    if (hk > hq || max_prefix_len > INT32_MAX || max_own_len > INT32_MAX || num_cu > kMax) return FCK_OK;
+    if (num_cu <= 0) num_cu = cu_count();
+    const auto choose = [&](int64_t streams, int64_t rows, int64_t keys) {
+        const int64_t items = streams * hk * ((rows + 63) / 64);
+        const int64_t want = (2 * num_cu + items - 1) / items, cap = keys / 256;
+        const int64_t ns = want < cap ? want : cap;
+        return (int32_t)(ns < 1 ? 1 : ns > 64 ? 64 : ns);
+    };
+    const int64_t g = hq / hk;
+    if (prefix_splits) *prefix_splits = choose(num_groups, max_group_size * sq * g, max_prefix_len);
+    if (own_splits) *own_splits = choose(batch, sq * g, max_own_len);
+    return FCK_OK;
+}
+
+int fck_fmha_decode_shared_prefix(const void* q, const void* k_cache, const void* v_cache, void* o, void* lse, void* lse_acc, void* o_acc,
+                                  const int32_t* seqstart_q, const int32_t* seqlen_k_ptr, const int32_t* block_table,
+                                  const int32_t* cu_groups, const int32_t* prefix_lens, int64_t batch, int64_t num_groups,
+                                  int64_t max_group_size, int64_t seqlen_q, int64_t hq, int64_t hk, int64_t d, int64_t dv,
+                                  int64_t q_max_seq_len, int64_t num_prefix_splits, int64_t num_own_splits,
+                                  int64_t batch_stride_block_table, int64_t page_block_size, float scale, int64_t window_left,
+                                  int64_t window_right, uint32_t mask_type, int32_t dtype, const fck_fmha_attrs* attrs, void* stream)
+{
+    g_err[0] = 0;
+    if (dtype == FCK_DTYPE_FP8) return fail(FCK_ERR_UNSUPPORTED, "shared-prefix decode takes fp16 or bf16 queries (an e4m3 cache goes through fck_fmha_attrs.kv_dtype)");
+    if (int rc = check_common(batch, hq, hk, d, dv, dtype)) return rc;
+    if (int rc = check_mask(mask_type)) return rc;
+    if (!q || !k_cache || !v_cache || !o || !lse_acc || !o_acc || !seqlen_k_ptr || !block_table || !prefix_lens)
+        return fail(FCK_ERR_INVALID_ARGUMENT, "q, k_cache, v_cache, o, lse_acc, o_acc, seqlen_k, block_table and prefix_lens must not be null");
+    if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(o) || !aligned16(o_acc))
+        return fail(FCK_ERR_INVALID_ARGUMENT, "q, k_cache, v_cache, o and o_acc must be 16-byte aligned");
+    if (!(scale > 0.f) || !std::isfinite(scale)) return fail(FCK_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
+    if (seqlen_q <= 0) return fail(FCK_ERR_INVALID_ARGUMENT, "seqlen_q must be positive (group mode: it carries total_q)");
+    if (q_max_seq_len <= 0) q_max_seq_len = seqlen_q;
+    if (num_groups < 1 || (!cu_groups && num_groups != 1)) return fail(FCK_ERR_INVALID_ARGUMENT, "num_groups must be positive, and 1 without cu_groups");
+    if (max_group_size <= 0 || max_group_size > batch) max_group_size = batch;
+    if (num_prefix_splits < 1 || num_prefix_splits > 64 || num_own_splits < 1 || num_own_splits > 64)
+        return fail(FCK_ERR_INVALID_ARGUMENT, "num_prefix_splits %ld / num_own_splits %ld out of range [1,64]", (long)num_prefix_splits, (long)num_own_splits);
+    if (page_block_size <= 0 || batch_stride_block_table <= 0) return fail(FCK_ERR_INVALID_ARGUMENT, "page_block_size and batch_stride_block_table must be positive");
+    if (int rc = check_fit32(page_block_size, batch_stride_block_table, seqlen_q, q_max_seq_len, num_groups, (seqstart_q ? 1 : batch) * seqlen_q)) return rc;
+    fck::SharedPrefixArgs a{};
+    a.q = q;
+    a.k = k_cache;
+    a.v = v_cache;
+    a.o = o;
+    a.lse = static_cast<float*>(lse);
+    a.lse_acc = static_cast<float*>(lse_acc);
+    a.o_acc = static_cast<float*>(o_acc);
+    a.seqstart_q = seqstart_q;
+    a.seqlen_k = seqlen_k_ptr;
+    a.block_table = block_table;
+    a.cu_groups = cu_groups;
+    a.prefix_lens = prefix_lens;
+    a.block_table_stride = (int32_t)batch_stride_block_table;
+    a.page_size = (int32_t)page_block_size;
+    a.page_shift = log2_exact(page_block_size);
+    a.batch = (int32_t)batch;
+    a.groups = (int32_t)num_groups;
+    a.max_group = (int32_t)max_group_size;
+    a.sq = (int32_t)seqlen_q;
+    a.hq = (int32_t)hq;
+    a.hk = (int32_t)hk;
+    a.d = (int32_t)d;
+    a.dv = (int32_t)dv;
+    a.ns_prefix = (int32_t)num_prefix_splits;
+    a.ns_own = (int32_t)num_own_splits;
+    a.shape_sq = seqlen_q;
+    a.scale_log2 = scale * fck::kLog2e;
+    a.mask_type = mask_type;
+    a.window_left = window_left;
+    a.window_right = window_right;
+    a.v_descale = 1.f;
+    a.num_cu = cu_count();
+    if (int rc = fill_mod(a.mod, nullptr, attrs, scale, mask_type, hq)) return rc;
+    if (a.mod.bias_type == FCK_BIAS_ELEMENTWISE) return fail(FCK_ERR_UNSUPPORTED, "shared-prefix decode takes ALiBi and the soft cap, not an elementwise bias");
+    if (int rc = only_score_attrs(attrs)) return rc;
+    if (int rc = fill_cache_type(a.kv8, a.scale_log2, a.mod, &a.v_descale, attrs, d, dv)) return rc;
+    const int64_t g = hq / hk;
+    g_kernel = "shared_prefix_kernel";
+    return launch_status(fck::launch_shared_prefix(a, kernel_dim(d, dv), dtype, max_group_size * q_max_seq_len * g, q_max_seq_len * g,
+                                                   static_cast<hipStream_t>(stream)), "shared-prefix decode launch");
+}
+
+int fck_fmha_key_weights(const void* q, const void* k, const void* lse, const void* weights, void* out, const int32_t* seqstart_q,
+                         const int32_t* seqlen_k_ptr, const int32_t* block_table, int64_t batch_stride_block_table,
+                         int64_t page_block_size, int64_t batch, int64_t seqlen_q, int64_t seqlen_k, int64_t cols, int64_t hq, int64_t hk,
+                         int64_t d, int64_t q_max_seq_len, float scale, int64_t window_left, int64_t window_right, uint32_t mask_type,
+                         int32_t dtype, const fck_fmha_attrs* attrs, void* stream)
+{
+    g_err[0] = 0;
+    if (dtype == FCK_DTYPE_FP8) return fail(FCK_ERR_UNSUPPORTED, "key weights take fp16 or bf16 queries (an e4m3 cache goes through fck_fmha_attrs.kv_dtype)");
+    if (int rc = check_common(batch, hq, hk, d, d, dtype)) return rc;
+    if (int rc = check_mask(mask_type)) return rc;
+    if (!q || !k || !lse || !out) return fail(FCK_ERR_INVALID_ARGUMENT, "q, k, lse and out must not be null");
+    if (!aligned16(q) || !aligned16(k)) return fail(FCK_ERR_INVALID_ARGUMENT, "q and k must be 16-byte aligned");
+    if (!(scale > 0.f) || !std::isfinite(scale)) return fail(FCK_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
+    if (seqlen_q <= 0) return fail(FCK_ERR_INVALID_ARGUMENT, "seqlen_q must be positive (group mode: it carries total_q)");
+    if (cols <= 0) return fail(FCK_ERR_INVALID_ARGUMENT, "cols (keys a row of the weights holds) must be positive");
+    if (q_max_seq_len <= 0) q_max_seq_len = seqlen_q;
+    if (int rc = check_fit32(seqlen_q, seqlen_k, q_max_seq_len, cols, batch_stride_block_table, page_block_size, (seqstart_q ? 1 : batch) * seqlen_q,
+                             q_max_seq_len * (hq / hk))) return rc;
+    fck::KeyWeightsArgs a{};
+    a.q = q;
+    a.k = k;
+    a.lse = static_cast<const float*>(lse);
+    a.weights = static_cast<const float*>(weights);
+    a.out = static_cast<float*>(out);
+    a.seqstart_q = seqstart_q;
+    a.kv.page_shift = -1;
+    a.kv.seqlen_k_ptr = seqlen_k_ptr;
+    if (block_table) {
+        if (page_block_size <= 0 || batch_stride_block_table <= 0) return fail(FCK_ERR_INVALID_ARGUMENT, "page_block_size and batch_stride_block_table must be positive");
+        if (!seqlen_k_ptr) return fail(FCK_ERR_INVALID_ARGUMENT, "paged cache needs per-sequence key counts");
+        a.kv.mode = 2;
+        a.kv.block_table = block_table;
+        a.kv.block_table_stride = (int32_t)batch_stride_block_table;
+        a.kv.page_size = (int32_t)page_block_size;
+        a.kv.page_shift = log2_exact(page_block_size);
+    } else {
+        if (seqlen_k <= 0) return fail(FCK_ERR_INVALID_ARGUMENT, "batch cache needs seqlen_k > 0");
+        a.kv.mode = 0;
+        a.kv.seqlen_k = (int32_t)seqlen_k;
+    }
+    a.cols = cols;
+    a.lse_sq = seqlen_q;
+    a.batch = (int32_t)batch;
+    a.sq = (int32_t)seqlen_q;
+    a.hq = (int32_t)hq;
+    a.hk = (int32_t)hk;
+    a.d = (int32_t)d;
+    a.scale_log2 = scale * fck::kLog2e;
+    a.mask_type = mask_type;
+    a.window_left = window_left;
+    a.window_right = window_right;
+    a.rows_max = (int32_t)(q_max_seq_len * (hq / hk));
+    a.num_cu = cu_count();
+    if (int rc = fill_mod(a.mod, nullptr, attrs, scale, mask_type, hq)) return rc;
+    if (a.mod.bias_type == FCK_BIAS_ELEMENTWISE) return fail(FCK_ERR_UNSUPPORTED, "key weights take ALiBi and the soft cap, not an elementwise bias");
+    if (int rc = only_score_attrs(attrs)) return rc;
+    if (int rc = fill_cache_type(a.kv8, a.scale_log2, a.mod, nullptr, attrs, d, d)) return rc;
+    g_kernel = "key_weights_kernel";
+    return launch_status(fck::launch_key_weights(a, kernel_dim(d, d), dtype, static_cast<hipStream_t>(stream)), "key-weights launch");
+}
+
+int fck_fmha_cache_evict(const void* k_cache, const void* v_cache, void* new_k_cache, void* new_v_cache, const void* weights,
+                         void* new_weights, const int32_t* seqlen_k, int32_t* new_seqlen_k, int32_t* kept, const int32_t* block_table,
+                         int64_t batch_stride_block_table, int64_t page_block_size, const int32_t* new_block_table,
+                         int64_t new_batch_stride_block_table, int64_t new_page_block_size, int64_t batch, int64_t hk, int64_t d, int64_t dv,
+                         int64_t cols, int64_t budget, int64_t recent, int64_t sinks, int32_t dtype, void* stream)
+{
+    g_err[0] = 0;
+    if (dtype != FCK_DTYPE_FP16 && dtype != FCK_DTYPE_BF16 && dtype != FCK_DTYPE_FP8)
+        return fail(FCK_ERR_UNSUPPORTED, "dtype %d: caches hold FLOAT8 (1, e4m3), FLOAT16 (3) or BFLOAT16 (4)", dtype);
+    if (!k_cache || !v_cache || !new_k_cache || !new_v_cache || !weights || !new_weights || !seqlen_k || !new_seqlen_k || !kept || !block_table || !new_block_table)
+        return fail(FCK_ERR_INVALID_ARGUMENT, "every pointer of the cache eviction must be given");
+    if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(new_k_cache) || !aligned16(new_v_cache))
+        return fail(FCK_ERR_INVALID_ARGUMENT, "the caches must be 16-byte aligned");
+    if (batch <= 0 || hk <= 0 || cols <= 0) return fail(FCK_ERR_INVALID_ARGUMENT, "batch, kv_num_heads and cols must be positive");
+    if (d < 8 || dv < 8 || d > 256 || dv > 256 || d % 8 || dv % 8)
+        return fail(FCK_ERR_UNSUPPORTED, "qk_head_dim %ld / v_head_dim %ld: head dims are multiples of 8 in [8, 256]", (long)d, (long)dv);
+    if (page_block_size <= 0 || batch_stride_block_table <= 0 || new_page_block_size <= 0 || new_batch_stride_block_table <= 0)
+        return fail(FCK_ERR_INVALID_ARGUMENT, "page sizes and block table strides must be positive");
+    if (int rc = check_fit32(batch, hk, cols, budget, page_block_size, batch_stride_block_table, new_page_block_size, new_batch_stride_block_table, batch * hk)) return rc;
+    if (budget <= 0 || recent < 0 || sinks < 0 || recent > budget || sinks > budget - recent)
+        return fail(FCK_ERR_INVALID_ARGUMENT, "budget %ld must be positive and hold recent %ld + sinks %ld", (long)budget, (long)recent, (long)sinks);
+    if (new_batch_stride_block_table * new_page_block_size < budget)
+        return fail(FCK_ERR_INVALID_ARGUMENT, "a row of new_block_table addresses %ld keys, the budget is %ld", (long)(new_batch_stride_block_table * new_page_block_size), (long)budget);
+    if (block_table == new_block_table && k_cache == new_k_cache)
+        return fail(FCK_ERR_INVALID_ARGUMENT, "new_block_table must name other pages than block_table: rows are not moved inside the pages that are read");
+    if (weights == new_weights) return fail(FCK_ERR_INVALID_ARGUMENT, "new_weights must not be weights");
+    const int e = dtype == FCK_DTYPE_FP8 ? 1 : 2;
+    fck::CacheEvictArgs a{};
+    a.k = k_cache;
+    a.v = v_cache;
+    a.new_k = new_k_cache;
+    a.new_v = new_v_cache;
+    a.weights = static_cast<const float*>(weights);
+    a.new_weights = static_cast<float*>(new_weights);
+    a.seqlen_k = seqlen_k;
+    a.new_seqlen = new_seqlen_k;
+    a.kept = kept;
+    a.block_table = block_table;
+    a.new_block_table = new_block_table;
+    a.block_table_stride = (int32_t)batch_stride_block_table;
+    a.new_block_table_stride = (int32_t)new_batch_stride_block_table;
+    a.page_size = (int32_t)page_block_size;
+    a.new_page_size = (int32_t)new_page_block_size;
+    a.batch = (int32_t)batch;
+    a.hk = (int32_t)hk;
+    a.budget = (int32_t)budget;
+    a.recent = (int32_t)recent;
+    a.sinks = (int32_t)sinks;
+    a.cols = cols;
+    a.k_row = (int32_t)(d * e);
+    a.v_row = (int32_t)(dv * e);
+    g_kernel = "evict_move_kernel";
+    return launch_status(fck::launch_cache_evict(a, static_cast<hipStream_t>(stream)), "cache eviction launch");
 }
 
 }  // extern "C"

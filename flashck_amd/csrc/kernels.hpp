@@ -63,6 +63,7 @@ struct CombineArgs {
     int32_t hq, dv, num_splits;
     int32_t num_cu;  // compute units of the device (decides the workgroup size)
     float o_scale;   // e4m3 output: O = saturate(o_scale * o)
+    float* lse;      // [Bs, Hq, Sq] log-sum-exp of every row, or null
 };
 
 struct AppendKvArgs {
@@ -105,7 +106,83 @@ struct PrefillArgs {
     float v_descale;  // factor on the output (1 unless V is quantised)
     int32_t q8;       // with kv8: Q and O are e4m3 too, P is rounded to e4m3 before the second product (all-fp8 roles)
     float o_scale;    // q8: O = saturate(o_scale * o)
+    float* lse;       // log-sum-exp of every row (natural log), or null: (b, h, i) at ((b * hq) + h) * lse_head_stride + i, packed
+    int64_t lse_head_stride;  // queries (h, row) at h * lse_head_stride + row
 };
+
+// Decode attention of a batch whose sequences share prefixes (shared_prefix.hip).
+struct SharedPrefixArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    void* o;
+    float* lse;      // [B, Hq, sq] or [Hq, total_q]; may be null
+    float* o_acc;    // partials [Bs, Hq, ns_prefix + ns_own, Sq, Dv], slots of the prefix splits first
+    float* lse_acc;  // [Bs, Hq, ns_prefix + ns_own, Sq]
+    const int32_t* seqstart_q;  // null: batch mode
+    const int32_t* seqlen_k;
+    const int32_t* block_table;
+    const int32_t* cu_groups;    // null: one group, the whole batch
+    const int32_t* prefix_lens;  // [groups]
+    int32_t block_table_stride, page_size, page_shift;
+    int32_t batch, groups, max_group;  // max_group: sequences of a group the prefix rows cover (the others read all of their own keys)
+    int32_t sq, hq, hk, d, dv;
+    int32_t ns_prefix, ns_own;
+    int32_t prefix_tiles, own_tiles;  // row tiles per (group, KV head) / per (sequence, KV head); set by the launcher
+    int32_t prefix_items;             // workgroups that handle prefixes; set by the launcher
+    int64_t shape_sq;                 // Sq of the workspace: sq (batch mode) or total_q
+    float scale_log2;
+    uint32_t mask_type;
+    int64_t window_left, window_right;
+    ScoreMod mod;  // ALiBi / soft cap
+    int32_t kv8;
+    float v_descale;
+    int32_t num_cu;
+};
+// rows_prefix / rows_own: most packed query rows of a group / of a sequence
+hipError_t launch_shared_prefix(SharedPrefixArgs a, int d, int dtype, int64_t rows_prefix, int64_t rows_own, hipStream_t st);
+
+// Attention weight every key of a cache receives (key_weights.hip).
+struct KeyWeightsArgs {
+    const void* q;
+    const void* k;
+    const float* lse;      // [B, Hq, sq] or [Hq, total_q]
+    const float* weights;  // [B, Hk, cols] or null; may be `out`
+    float* out;            // [B, Hk, cols]
+    const int32_t* seqstart_q;
+    KvAddr kv;
+    int64_t cols;
+    int64_t lse_sq;  // row length of lse: sq or total_q
+    int32_t batch, sq, hq, hk, d;
+    float scale_log2;
+    uint32_t mask_type;
+    int64_t window_left, window_right;
+    ScoreMod mod;  // ALiBi / soft cap
+    int32_t kv8;
+    int32_t rows_max;  // most packed query rows of a sequence
+    int32_t num_cu;
+};
+hipError_t launch_key_weights(const KeyWeightsArgs& a, int d, int dtype, hipStream_t st);
+
+// Choice of the keys a cache keeps, and their move to new pages (cache_evict.hip).
+struct CacheEvictArgs {
+    const void* k;
+    const void* v;
+    void* new_k;
+    void* new_v;
+    const float* weights;  // [B, Hk, cols]
+    float* new_weights;    // [B, Hk, cols]
+    const int32_t* seqlen_k;
+    int32_t* new_seqlen;  // [B]
+    int32_t* kept;        // [B, Hk, budget]
+    const int32_t* block_table;
+    const int32_t* new_block_table;
+    int32_t block_table_stride, new_block_table_stride, page_size, new_page_size;
+    int32_t batch, hk, budget, recent, sinks;
+    int64_t cols;
+    int32_t k_row, v_row;  // bytes of one head's row of K and V (multiples of 8)
+};
+hipError_t launch_cache_evict(const CacheEvictArgs& a, hipStream_t st);
 
 // arguments of the paged-cache checker: a block table (block_table != nullptr: seqlen_k, block_table_stride) or a page
 // list (kv_indptr, kv_page_indices, optional kv_last_page_lens)

@@ -338,6 +338,9 @@ __global__ __launch_bounds__(256, (D == 256 ? 1 : 2)) void prefill_kernel(const 
     // ---- epilogue ----------------------------------------------------------------------------------------------------
     l_run = pair32_sum(l_run);
     if (row_ok) {
+        if (a.lse != nullptr && half == 0)
+            a.lse[((int64_t)(a.seqstart_q ? 0 : b) * a.hq + h) * a.lse_head_stride + (a.seqstart_q ? q_row0 : 0) + r] =
+                l_run == 0.f ? -INFINITY : (m_run + fast_log2(l_run)) * kLn2;
         float inv = (l_run == 0.f) ? 0.f : 1.f / l_run;
         if constexpr (kKv8) inv *= a.v_descale;
         if constexpr (kKv8) {

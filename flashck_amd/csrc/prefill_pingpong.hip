@@ -458,6 +458,9 @@ __global__ __launch_bounds__(512) void prefill_pp_kernel(const PrefillArgs a)
     // ---- epilogue ----------------------------------------------------------------------------------------------------
     l_run = pair32_sum(l_run);
     if (row_ok) {
+        if (a.lse != nullptr && half == 0)
+            a.lse[((int64_t)(a.seqstart_q ? 0 : b) * a.hq + h) * a.lse_head_stride + (a.seqstart_q ? q_row0 : 0) + r] =
+                l_run == 0.f ? -INFINITY : (m_run + fast_log2(l_run)) * kLn2;
         const float inv = (l_run == 0.f) ? 0.f : 1.f / l_run;
         uint16_t* op = reinterpret_cast<uint16_t*>(a.o) + ((int64_t)(q_row0 + r) * a.hq + h) * dvs;
 #pragma unroll

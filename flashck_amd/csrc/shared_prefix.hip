@@ -1,0 +1,433 @@
+// Decode attention of a batch whose sequences share prefixes (gfx950).
+//
+// The sequences [c_g, c_{g+1}) of group g begin with the same P_g tokens.  Softmax attention over a union of disjoint key
+// sets is the merge of the attentions over each of them,
+//   LSE = log(sum_s exp(LSE_s)),  O = sum_s exp(LSE_s - LSE) O_s,
+// so the keys of a prefix are attended to by the query rows of the whole group at once (they are read once, through the
+// pages of the group's first sequence) and the keys behind it by the rows of each sequence alone.  One launch does both,
+// a second one merges the partial results.
+//
+// Work decomposition
+//   An item = a tile of packed query rows (token, head of the KV head's group) x one split of a key range: of a prefix with
+//   the rows of its group, or of a sequence's own keys with the rows of that sequence.  Which keys a row sees is a range
+//   [lo, hi) of its own (its sequence's length and mask decide), so an item never has to know where its rows come from
+//   after it has set them up.
+//   Prefix items come first (they are the long ones); those that stream the same keys get ids congruent modulo 8, i.e. one
+//   XCD and one L2.
+#include "common.hpp"
+#include "kernels.hpp"
+
+namespace fck {
+namespace {
+
+struct SharedGroup {
+    int first, count, prefix;
+};
+
+__device__ __forceinline__ int shared_len(const SharedPrefixArgs& a, int b)
+{
+    const int64_t cap = (int64_t)a.block_table_stride * a.page_size;
+    const int n = max(a.seqlen_k[b], 0);
+    return n < cap ? n : (int)cap;
+}
+
+// sequences [first, first + count) of group g share their first `prefix` tokens (never more than the first of them has)
+__device__ __forceinline__ SharedGroup shared_group(const SharedPrefixArgs& a, int g)
+{
+    SharedGroup s;
+    s.first = a.cu_groups ? min(max(a.cu_groups[g], 0), a.batch) : 0;
+    const int end = a.cu_groups ? min(max(a.cu_groups[g + 1], s.first), a.batch) : a.batch;
+    s.count = min(end - s.first, a.max_group);
+    s.prefix = s.count > 0 ? min(max(a.prefix_lens[g], 0), shared_len(a, s.first)) : 0;
+    return s;
+}
+
+// number of entries of the non-decreasing starts[0..n] that are <= x, minus one: the interval x lies in
+__device__ __forceinline__ int interval_of(const int32_t* starts, int n, int x)
+{
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (starts[mid] <= x)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    return lo;
+}
+
+// first key of sequence b that is not part of its group's prefix
+__device__ __forceinline__ int own_begin(const SharedPrefixArgs& a, int b)
+{
+    const SharedGroup s = shared_group(a, a.cu_groups ? interval_of(a.cu_groups, a.groups, b) : 0);
+    return b >= s.first && b < s.first + s.count ? s.prefix : 0;
+}
+
+template <int D>
+struct SharedShape {
+    static constexpr int TK = D == 256 ? 32 : 64;  // keys per tile
+    static constexpr int BM = 64;                  // query rows per workgroup, 16 per wave
+    static constexpr int NBK = TK / 16;            // 16-key blocks per tile
+    static constexpr int KT = D / 32;              // MFMA k-steps of the QK product
+    static constexpr int DB = D / 16;              // 16-column blocks of the output
+    static constexpr int CH = D / 8;               // 16-byte chunks per staged row
+    static constexpr int ROWB = D * 2;
+    static constexpr int TILEB = TK * ROWB;
+    static constexpr int LD = TK * CH / 256;  // chunks per thread and operand
+};
+
+template <int D>
+__device__ __forceinline__ int shared_v_swizzle(int key)
+{
+    return ((key & 7) << 1) & (D / 8 - 1);
+}
+
+// The kernel for every head dim, page size and cache type: 4 waves of 16 rows, K/V tiles through registers into
+// double-buffered LDS that all waves read.
+// kUniform: pages are a multiple of the key tile.  kMod: ALiBi / soft cap.  kPad: stored head dims smaller than D (missing
+// chunks are zeros).  kKv8: e4m3 caches, widened to T on their way into LDS; always with kMod.
+template <typename T, int D, bool kUniform, bool kMod, bool kPad, bool kKv8>
+__global__ __launch_bounds__(256) void shared_prefix_kernel(const SharedPrefixArgs a)
+{
+    typedef SharedShape<D> S;
+    typedef typename T::vec8 vec8;
+    FCK_DYNAMIC_LDS(smem);
+    char FCK_LDS* const lds = (char FCK_LDS*)smem;  // K0 | K1 | V0 | V1 | visible range
+    int FCK_LDS* const range = (int FCK_LDS*)(lds + 4 * S::TILEB);
+
+    const int dq = kPad ? a.d : D, dvs = kPad ? a.dv : D;
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, kg = lane >> 4;
+    const int g = a.hq / a.hk;
+
+    // ---- the item (uniform) ----------------------------------------------------------------------------------------------
+    int id = blockIdx.x;
+    const bool prefix = id < a.prefix_items;
+    int hkv, split, ns, slot, mt, leader, key_lo, key_hi, tok0, tok1;
+    if (prefix) {
+        constexpr int kXcd = 8;
+        const int s = id / kXcd;
+        mt = s % a.prefix_tiles;
+        const int stream = s / a.prefix_tiles * kXcd + id % kXcd;
+        if (stream >= a.groups * a.ns_prefix * a.hk) return;
+        hkv = stream % a.hk;
+        split = slot = stream / a.hk % a.ns_prefix;
+        ns = a.ns_prefix;
+        const SharedGroup sg = shared_group(a, stream / (a.hk * a.ns_prefix));
+        leader = sg.first;
+        key_lo = 0;
+        key_hi = sg.prefix;
+        if (key_hi <= 0) return;
+        tok0 = a.seqstart_q ? a.seqstart_q[sg.first] : sg.first * a.sq;
+        tok1 = a.seqstart_q ? a.seqstart_q[sg.first + sg.count] : (sg.first + sg.count) * a.sq;
+    } else {
+        id -= a.prefix_items;
+        hkv = id % a.hk;
+        id /= a.hk;
+        split = id % a.ns_own;
+        id /= a.ns_own;
+        mt = id % a.own_tiles;
+        const int b = leader = id / a.own_tiles;
+        ns = a.ns_own;
+        slot = a.ns_prefix + split;
+        key_lo = own_begin(a, b);
+        key_hi = shared_len(a, b);
+        if (key_hi <= key_lo) return;
+        tok0 = a.seqstart_q ? a.seqstart_q[b] : b * a.sq;
+        tok1 = a.seqstart_q ? a.seqstart_q[b + 1] : tok0 + a.sq;
+    }
+    const int64_t R = (int64_t)(tok1 - tok0) * g;
+    const int64_t r0 = (int64_t)mt * S::BM;
+    if (r0 >= R) return;
+    // splits are equal runs of whole tiles
+    const int base = key_lo / S::TK * S::TK;
+    const int64_t per = ((int64_t)(key_hi - base) + (int64_t)ns * S::TK - 1) / ((int64_t)ns * S::TK) * S::TK;
+    const int k0 = (int)min(max((int64_t)key_lo, base + per * split), (int64_t)key_hi);
+    const int k1 = (int)min((int64_t)key_hi, base + per * (split + 1));
+
+    // ---- this lane's row ---------------------------------------------------------------------------------------------------
+    const int64_t r = r0 + wave * 16 + l16;
+    const bool row_ok = r < R;
+    const int tok = tok0 + (row_ok ? (int)(r / g) : 0);
+    const int h = hkv * g + (row_ok ? (int)(r % g) : 0);
+    const int b = !prefix ? leader : a.seqstart_q ? interval_of(a.seqstart_q, a.batch, tok) : tok / a.sq;
+    const int first_tok = a.seqstart_q ? a.seqstart_q[b] : b * a.sq;
+    const int sq_b = a.seqstart_q ? a.seqstart_q[b + 1] - first_tok : a.sq;
+    const int i = tok - first_tok;
+    const int sk_b = shared_len(a, b);
+    const MaskYX mk = make_mask(a.mask_type, a.window_left, a.window_right, sq_b, sk_b);
+    const int lo = row_ok ? max(mask_lo(mk, i), k0) : 0;
+    const int hi = row_ok ? min(mask_hi(mk, i, sk_b), k1) : 0;
+    ArithMod amod;
+    if constexpr (kMod) amod.init(a.mod, b, h, i, sq_b, sk_b, a.mask_type, a.window_left, a.window_right);
+    // place of the row's partial result
+    const int64_t wrow = ((int64_t)(a.seqstart_q ? 0 : b) * a.hq + h) * (a.ns_prefix + a.ns_own) + slot;
+    const int64_t wofs = wrow * a.shape_sq + (a.seqstart_q ? tok : i);
+
+    // keys any row of the workgroup sees
+    if (tid == 0) {
+        range[0] = INT32_MAX;
+        range[1] = 0;
+    }
+    __syncthreads();
+    if (lo < hi && kg == 0) {
+        atomicMin((int*)&range[0], lo);
+        atomicMin((int*)&range[1], -hi);
+    }
+    __syncthreads();
+    const int vis_lo = range[0], vis_hi = -range[1];
+    if (vis_lo >= vis_hi) {  // an empty split, or one that every row's mask leaves out
+        if (row_ok && kg == 0) a.lse_acc[wofs] = -INFINITY;
+        return;
+    }
+    const int t_begin = vis_lo / S::TK;
+    const int n = (vis_hi + S::TK - 1) / S::TK - t_begin;
+    const bool wave_rows = r0 + wave * 16 < R;  // uniform
+
+    vec8 qf[S::KT];
+    {
+        const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + ((int64_t)tok * a.hq + h) * dq + kg * 8;
+#pragma unroll
+        for (int t = 0; t < S::KT; ++t) {
+            u32x4_t v = {0u, 0u, 0u, 0u};
+            if (row_ok && (!kPad || t * 32 + kg * 8 < dq)) v = ldg16(qp + t * 32);
+            qf[t] = as_vec8<vec8>(v);
+        }
+    }
+    float m_run = -INFINITY, l_run = 0.f;
+    f32x4_t oacc[S::DB];
+#pragma unroll
+    for (int db = 0; db < S::DB; ++db) oacc[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+    // ---- K/V tiles ----------------------------------------------------------------------------------------------------------
+    const int32_t* table = a.block_table + (int64_t)leader * a.block_table_stride;
+    auto page_of = [&](int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / a.page_size; };
+    auto cache_row = [&](int key) -> int64_t {
+        const int pi = page_of(key);
+        return (int64_t)table[pi] * a.page_size + (key - pi * a.page_size);
+    };
+    constexpr int kElem = kKv8 ? 1 : 2;
+    auto fetch = [&](const void* base_p, int64_t row, int chunk, int dim) -> u32x4_t {
+        if (kPad && chunk * 8 >= dim) return u32x4_t{0u, 0u, 0u, 0u};
+        const char* p = (const char*)base_p + ((row * a.hk + hkv) * dim + chunk * 8) * kElem;
+        if constexpr (kKv8) {
+            const u32x2_t v = *reinterpret_cast<const u32x2_t*>(p);
+            return u32x4_t{v[0], v[1], 0u, 0u};
+        } else {
+            return ldg16(p);
+        }
+    };
+    auto staged = [](u32x4_t v) -> u32x4_t {
+        if constexpr (kKv8)
+            return fp8x8_to_t<T>(v);
+        else
+            return v;
+    };
+    u32x4_t kreg[S::LD], vreg[S::LD];
+    auto load_tile = [&](int c) {
+        const int kb = (t_begin + c) * S::TK;
+        int64_t row0 = 0;
+        if constexpr (kUniform) row0 = cache_row(kb);
+#pragma unroll
+        for (int u = 0; u < S::LD; ++u) {
+            const int row = (u * 256 + tid) / S::CH, chunk = (u * 256 + tid) % S::CH;
+            // rows outside the item's keys repeat its first or last one (their scores are masked)
+            const int key = min(max(kb + row, key_lo), key_hi - 1);
+            const int64_t cr = kUniform ? row0 + (key - kb) : cache_row(key);
+            kreg[u] = fetch(a.k, cr, chunk, dq);
+            vreg[u] = fetch(a.v, cr, chunk, dvs);
+        }
+    };
+    auto store_tile = [&](int buf) {
+#pragma unroll
+        for (int u = 0; u < S::LD; ++u) {
+            const int row = (u * 256 + tid) / S::CH, chunk = (u * 256 + tid) % S::CH;
+            *(u32x4_t FCK_LDS*)(lds + buf * S::TILEB + row * S::ROWB + ((chunk ^ (row & 7)) << 4)) = staged(kreg[u]);
+            *(u32x4_t FCK_LDS*)(lds + (2 + buf) * S::TILEB + row * S::ROWB + ((chunk ^ shared_v_swizzle<D>(row)) << 4)) = staged(vreg[u]);
+        }
+    };
+
+    const int tr_key = kg * 4 + (l16 >> 2);
+    const int tr_sw = shared_v_swizzle<D>(tr_key);
+    const int tr_base = tr_key * S::ROWB + ((l16 & 2) << 3) + ((l16 & 1) << 3);
+    auto compute = [&](int c, int buf) {
+        const int kb = (t_begin + c) * S::TK;
+        const char FCK_LDS* kt = lds + buf * S::TILEB + l16 * S::ROWB;
+        const char FCK_LDS* vt = lds + (2 + buf) * S::TILEB + tr_base;
+        // S^T[key][row] = K . Q^T
+        float x[4 * S::NBK];
+        float tmax = -INFINITY;
+#pragma unroll
+        for (int nb = 0; nb < S::NBK; ++nb) {
+            f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int t = 0; t < S::KT; ++t) {
+                const u32x4_t kf = *(const u32x4_t FCK_LDS*)(kt + nb * 16 * S::ROWB + (((t * 4 + kg) ^ (l16 & 7)) << 4));
+                acc = T::mfma16(as_vec8<vec8>(kf), qf[t], acc);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int key = kb + nb * 16 + kg * 4 + j;
+                const bool vis = key >= lo && key < hi;
+                float v;
+                if constexpr (kMod)
+                    v = vis ? amod.score(acc[j], key) : -INFINITY;
+                else
+                    v = vis ? acc[j] * a.scale_log2 : -INFINITY;
+                x[nb * 4 + j] = v;
+                tmax = fmaxf(tmax, v);
+            }
+        }
+        tmax = quad16_max(tmax);
+        const float m_new = fmaxf(m_run, tmax);
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = fast_exp2(m_run - m_use);
+        m_run = m_new;
+        float psum = 0.f;
+        uint32_t pk[2 * S::NBK];
+#pragma unroll
+        for (int e = 0; e < 2 * S::NBK; ++e) {
+            const float p0 = fast_exp2(x[2 * e] - m_use), p1 = fast_exp2(x[2 * e + 1] - m_use);
+            psum += p0 + p1;
+            // P feeds the 16-bit matrix instructions like K and V do; the row sum keeps the unrounded values
+            pk[e] = T::pack2(p0, p1);
+        }
+        l_run = l_run * alpha + psum;
+#pragma unroll
+        for (int db = 0; db < S::DB; ++db) oacc[db] *= alpha;
+        // O^T[dv][row] += V^T . P^T
+#pragma unroll
+        for (int kk = 0; kk < S::NBK / 2; ++kk) {
+            const u32x4_t pv = {pk[kk * 4], pk[kk * 4 + 1], pk[kk * 4 + 2], pk[kk * 4 + 3]};
+#pragma unroll
+            for (int db = 0; db < S::DB; ++db) {
+                const char FCK_LDS* p = vt + kk * 32 * S::ROWB + (((db * 2) ^ tr_sw) << 4);
+                const u32x2_t lo4 = lds_read_tr16(p), hi4 = lds_read_tr16(p + 16 * S::ROWB);
+                const u32x4_t av = {lo4[0], lo4[1], hi4[0], hi4[1]};
+                oacc[db] = T::mfma16(as_vec8<vec8>(av), as_vec8<vec8>(pv), oacc[db]);
+            }
+        }
+    };
+
+    // tile c is in LDS buffer c % 2 behind the barrier of iteration c; tile c + 1 is in flight meanwhile
+    load_tile(0);
+    for (int c = 0; c < n; ++c) {
+        store_tile(c & 1);
+        __syncthreads();
+        if (c + 1 < n) load_tile(c + 1);
+        if (wave_rows) compute(c, c & 1);
+    }
+
+    l_run = quad16_sum(l_run);
+    if (!row_ok) return;
+    const float inv = l_run == 0.f ? 0.f : a.v_descale / l_run;
+    float* op = a.o_acc + wofs * dvs + kg * 4;
+#pragma unroll
+    for (int db = 0; db < S::DB; ++db) {
+        if (kPad && db * 16 + kg * 4 >= dvs) continue;
+        *reinterpret_cast<f32x4_t*>(op + db * 16) = oacc[db] * inv;
+    }
+    if (kg == 0) a.lse_acc[wofs] = l_run == 0.f ? -INFINITY : (m_run + fast_log2(l_run)) * kLn2;
+}
+
+// Merge of a row's partial results: the prefix splits if its sequence has a shared prefix, the own splits if it has keys
+// behind it.  Dv/4 lanes per row, 4 columns each.
+template <typename T, int DV>
+__global__ __launch_bounds__(256) void shared_prefix_combine_kernel(const SharedPrefixArgs a)
+{
+    constexpr int TPR = DV / 4;
+    const int64_t item = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;  // (row, head)
+    const int c = threadIdx.x % TPR * 4;
+    const int64_t rows = a.seqstart_q ? a.shape_sq : (int64_t)a.batch * a.sq;
+    if (item >= rows * a.hq || c >= a.dv) return;
+    const int tok = (int)(item / a.hq), h = (int)(item % a.hq);
+    int b, i;
+    if (a.seqstart_q) {
+        b = interval_of(a.seqstart_q, a.batch, tok);
+        if (tok >= a.seqstart_q[b + 1] || tok < a.seqstart_q[b]) return;  // a row behind the last sequence stays as it was
+        i = tok;
+    } else {
+        b = tok / a.sq;
+        i = tok - b * a.sq;
+    }
+    const int own = own_begin(a, b), len = shared_len(a, b);
+    const int first = own > 0 ? 0 : a.ns_prefix;
+    const int last = len > own ? a.ns_prefix + a.ns_own : a.ns_prefix;
+    const int64_t w0 = (((int64_t)(a.seqstart_q ? 0 : b) * a.hq + h) * (a.ns_prefix + a.ns_own) + first) * a.shape_sq + i;
+    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+    if (last > first) acc = combine_splits<DV>(a.lse_acc, a.o_acc, w0, a.shape_sq, last - first, c, a.dv);
+    u32x2_t out;
+    out[0] = T::pack2(acc[0], acc[1]);
+    out[1] = T::pack2(acc[2], acc[3]);
+    *reinterpret_cast<u32x2_t*>(reinterpret_cast<uint16_t*>(a.o) + item * a.dv + c) = out;
+    if (a.lse && c == 0)
+        a.lse[((int64_t)(a.seqstart_q ? 0 : b) * a.hq + h) * a.shape_sq + i] = combine_lse(a.lse_acc, w0, a.shape_sq, last - first);
+}
+
+template <typename T, int D>
+hipError_t launch_general(const SharedPrefixArgs& a, bool uniform, int64_t grid, hipStream_t st)
+{
+    constexpr size_t lds = (size_t)4 * SharedShape<D>::TILEB + 16;
+    const dim3 blocks((unsigned)grid), threads(256);
+    if (a.kv8) {
+        if (uniform) return launch_with_lds<shared_prefix_kernel<T, D, true, true, false, true>>(blocks, threads, lds, st, a);
+        return launch_with_lds<shared_prefix_kernel<T, D, false, true, false, true>>(blocks, threads, lds, st, a);
+    }
+    if (a.d != D || a.dv != D) {
+        if (uniform) return launch_with_lds<shared_prefix_kernel<T, D, true, true, true, false>>(blocks, threads, lds, st, a);
+        return launch_with_lds<shared_prefix_kernel<T, D, false, true, true, false>>(blocks, threads, lds, st, a);
+    }
+    if (a.mod.active()) {
+        if (uniform) return launch_with_lds<shared_prefix_kernel<T, D, true, true, false, false>>(blocks, threads, lds, st, a);
+        return launch_with_lds<shared_prefix_kernel<T, D, false, true, false, false>>(blocks, threads, lds, st, a);
+    }
+    if (uniform) return launch_with_lds<shared_prefix_kernel<T, D, true, false, false, false>>(blocks, threads, lds, st, a);
+    return launch_with_lds<shared_prefix_kernel<T, D, false, false, false, false>>(blocks, threads, lds, st, a);
+}
+
+template <typename T, int DV>
+hipError_t launch_combine(const SharedPrefixArgs& a, hipStream_t st)
+{
+    const int64_t items = (a.seqstart_q ? a.shape_sq : (int64_t)a.batch * a.sq) * a.hq;
+    constexpr int per_wg = 256 / (DV / 4);
+    const int64_t grid = (items + per_wg - 1) / per_wg;
+    if (grid > INT32_MAX) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((shared_prefix_combine_kernel<T, DV>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
+template <typename T, int D>
+hipError_t launch_d(SharedPrefixArgs& a, int64_t rows_prefix, int64_t rows_own, hipStream_t st)
+{
+    constexpr int BM = SharedShape<D>::BM;
+    const int64_t p_tiles = (rows_prefix + BM - 1) / BM, o_tiles = (rows_own + BM - 1) / BM;
+    const int64_t streams = ((int64_t)a.groups * a.ns_prefix * a.hk + 7) / 8 * 8;
+    const int64_t prefix_items = streams * p_tiles;
+    const int64_t grid = prefix_items + (int64_t)a.hk * a.ns_own * o_tiles * a.batch;
+    if (p_tiles > INT32_MAX || o_tiles > INT32_MAX || grid > INT32_MAX) return hipErrorInvalidValue;
+    a.prefix_tiles = (int32_t)p_tiles;
+    a.own_tiles = (int32_t)o_tiles;
+    a.prefix_items = (int32_t)prefix_items;
+    // a key tile then never straddles a page
+    const bool uniform = a.page_size % SharedShape<D>::TK == 0;
+    if (hipError_t e = launch_general<T, D>(a, uniform, grid, st); e != hipSuccess) return e;
+    if (a.dv <= 64) return launch_combine<T, 64>(a, st);
+    if (a.dv <= 128) return launch_combine<T, 128>(a, st);
+    return launch_combine<T, 256>(a, st);
+}
+
+}  // namespace
+
+hipError_t launch_shared_prefix(SharedPrefixArgs a, int d, int dtype, int64_t rows_prefix, int64_t rows_own, hipStream_t st)
+{
+    switch (d) {
+    case 64: return dtype == 4 ? launch_d<BF16, 64>(a, rows_prefix, rows_own, st) : launch_d<FP16, 64>(a, rows_prefix, rows_own, st);
+    case 128: return dtype == 4 ? launch_d<BF16, 128>(a, rows_prefix, rows_own, st) : launch_d<FP16, 128>(a, rows_prefix, rows_own, st);
+    case 256: return dtype == 4 ? launch_d<BF16, 256>(a, rows_prefix, rows_own, st) : launch_d<FP16, 256>(a, rows_prefix, rows_own, st);
+    }
+    return hipErrorInvalidValue;
+}
+
+}  // namespace fck

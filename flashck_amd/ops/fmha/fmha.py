@@ -11,6 +11,7 @@ Tensor conventions (T = torch.float16 | torch.bfloat16, contiguous, on the GPU):
     k/v_cache    paged [num_pages, page_size, Hk, D] with block_table int32 [B, max_pages_per_seq]
     seqlen_k     int32 [B] valid keys per sequence
 """
+import contextlib
 import ctypes
 import math
 from typing import Optional, Tuple
@@ -26,6 +27,7 @@ __all__ = [
     "fmha_fwd_splitkv_fused", "fused_splitkv_fits",
     "fmha_fwd_appendkv", "fmha_batch_prefill", "fmha_fwd_pagedkv", "fmha_decode_paged", "fmha_decode_step",
     "tune_decode_num_splits", "tune_prefill_variant", "DecodeWorkspace", "num_splits_heuristic", "splitkv_workspace", "validate_paged", "fused_reset",
+    "fmha_decode_shared_prefix", "fmha_key_weights", "fmha_cache_evict", "shared_prefix_splits",
 ]
 
 # GenericAttentionMaskEnum / RopeEnum, core/profiling/attention/fmha_library.h:81-87,195-200
@@ -125,11 +127,12 @@ def _window(window):
 
 
 def _attrs(q, bias, alibi_slopes, logits_soft_cap, group, batch, rows, min_cols, kv_fp8=False, k_descale=1.0, v_descale=1.0,
-           decode_variant=0, prefill_variant=0, max_seqlen_k=0, o_scale=1.0):
+           decode_variant=0, prefill_variant=0, max_seqlen_k=0, o_scale=1.0, lse=None):
     """fck_fmha_attrs for a call, or None when no score modifier is asked for.
 
     o_scale (float8_e4m3fn queries on the dense / paged / page-list prefill calls): the output is
     saturate(o_scale * o) in e4m3.
+    lse: fp32 [B, Hq, sq] (group mode [Hq, total_q]) that receives the log-sum-exp of every row, on the prefill-family calls.
     bias (elementwise, BiasEnum ELEMENTWISE_BIAS): q's dtype (float32 for float8_e4m3fn queries), last dim contiguous; batch mode [1|B, 1|Hq, sq, >= sk],
     group mode [1|Hq, total_q, >= max sk]; size-1 dims are shared (the reference's rank 0 / 1 / 2).
     alibi_slopes (ALIBI): fp32 [Hq] or [B, Hq].  logits_soft_cap > 0: s = cap * tanh(scale * qk / cap).
@@ -142,7 +145,7 @@ def _attrs(q, bias, alibi_slopes, logits_soft_cap, group, batch, rows, min_cols,
                          "with splits of equal size in keys)")
     if int(prefill_variant) not in (0, 1, 2, 3, 4):
         raise ValueError("prefill_variant must be 0 (library's choice) or 1..4 (see fck_fmha_attrs.prefill_variant)")
-    if bias is None and alibi_slopes is None and cap == 0.0 and not kv_fp8 and not decode_variant and not prefill_variant:
+    if bias is None and alibi_slopes is None and cap == 0.0 and not kv_fp8 and not decode_variant and not prefill_variant and lse is None:
         return None, None
     if bias is not None and alibi_slopes is not None:
         raise ValueError("bias and alibi_slopes are exclusive (one BiasEnum per call)")
@@ -160,6 +163,10 @@ def _attrs(q, bias, alibi_slopes, logits_soft_cap, group, batch, rows, min_cols,
         raise ValueError("o_scale must be positive and finite")
     a.o_scale = float(o_scale)
     Hq = q.shape[-2]
+    if lse is not None:
+        _check_tensor("lse", lse, dtype=torch.float32)
+        _check_shape("lse", lse, (Hq, rows) if group else (batch, Hq, rows), q)
+        a.lse, a.lse_head_stride = lse.data_ptr(), rows
     if bias is not None:
         if not isinstance(bias, torch.Tensor):
             raise TypeError(f"Expected bias to be a torch.Tensor, got {type(bias)}")
@@ -188,7 +195,7 @@ def _attrs(q, bias, alibi_slopes, logits_soft_cap, group, batch, rows, min_cols,
         a.bias_type = 2
         a.bias = alibi_slopes.data_ptr()
         a.bias_batch_stride = Hq if alibi_slopes.dim() == 2 else 0
-    return ctypes.byref(a), (a, bias, alibi_slopes)
+    return ctypes.byref(a), (a, bias, alibi_slopes, lse)
 
 
 def validate_paged(*, seqlen_k=None, block_table=None, kv_indptr=None, kv_page_indices=None, kv_last_page_lens=None,
@@ -252,10 +259,11 @@ def splitkv_workspace(shape_batch, q_num_heads, shape_seqlen_q, v_head_dim, num_
 
 def fmha_fwd(q, k, v, scale: float = 0.0, mask_type: int = MASK_NONE, window: Tuple[int, int] = (-1, -1),
              seqlen_k: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, *, bias=None, alibi_slopes=None,
-             logits_soft_cap: float = 0.0, k_descale: float = 1.0, v_descale: float = 1.0, o_scale: float = 1.0) -> torch.Tensor:
+             logits_soft_cap: float = 0.0, k_descale: float = 1.0, v_descale: float = 1.0, o_scale: float = 1.0, lse=None) -> torch.Tensor:
     """Dense attention, batch mode: q [B,sq,Hq,D], k/v [B,sk,Hk,D] -> o [B,sq,Hq,D].
     bias / alibi_slopes / logits_soft_cap: see _attrs.  float8_e4m3fn tensors: the all-fp8 roles, with k = k_descale *
-    stored, v = v_descale * stored, o = saturate(o_scale * result)."""
+    stored, v = v_descale * stored, o = saturate(o_scale * result).  lse (fp32 [B,Hq,sq], optional) receives the log-sum-exp
+    of every row."""
     _check_tensor("q", q, ndim=4)
     _check_tensor("k", k, dtype=q.dtype, ndim=4)
     _check_tensor("v", v, dtype=q.dtype, ndim=4)
@@ -272,7 +280,7 @@ def fmha_fwd(q, k, v, scale: float = 0.0, mask_type: int = MASK_NONE, window: Tu
     o = _out("out", out, (B, sq, Hq, Dv), q.dtype, q)
     wl, wr = _window(window)
     at, keep = _attrs(q, bias, alibi_slopes, logits_soft_cap, False, B, sq, sk, q.dtype == torch.float8_e4m3fn, k_descale, v_descale,
-                      o_scale=o_scale)
+                      o_scale=o_scale, lse=lse)
     if at is None:
         _call("fck_fmha_fwd", _ptr(q), _ptr(k), _ptr(v), None, _ptr(o), None, None, _ptr(seqlen_k), B, sq, sk, Hq, Hk, D, Dv,
               sq, _scale(scale, D), wl, wr, mask_type, _dtype_id(q), _stream())
@@ -285,9 +293,10 @@ def fmha_fwd(q, k, v, scale: float = 0.0, mask_type: int = MASK_NONE, window: Tu
 
 def fmha_fwd_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q: int, scale: float = 0.0,
                     mask_type: int = MASK_NONE, window=(-1, -1), seqlen_k=None, out=None, *, bias=None, alibi_slopes=None,
-                    logits_soft_cap: float = 0.0, k_descale: float = 1.0, v_descale: float = 1.0, o_scale: float = 1.0) -> torch.Tensor:
+                    logits_soft_cap: float = 0.0, k_descale: float = 1.0, v_descale: float = 1.0, o_scale: float = 1.0, lse=None) -> torch.Tensor:
     """Dense attention, group mode: q [total_q,Hq,D], k/v [total_k,Hk,D] packed by cu_seqlens.
     bias / alibi_slopes / logits_soft_cap: see _attrs; float8_e4m3fn tensors and their scales: see fmha_fwd.
+    lse (fp32 [Hq,total_q], optional) receives the log-sum-exp of every row.
 
     seqlen_k (int32 [B], optional): logical key counts when the packed K/V slots hold padding behind the keys."""
     _check_tensor("q", q, ndim=3)
@@ -307,7 +316,7 @@ def fmha_fwd_varlen(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q: int, scal
     o = _out("out", out, (tq, Hq, Dv), q.dtype, q)
     wl, wr = _window(window)
     at, keep = _attrs(q, bias, alibi_slopes, logits_soft_cap, True, B, tq, 1, q.dtype == torch.float8_e4m3fn, k_descale, v_descale,
-                      o_scale=o_scale)
+                      o_scale=o_scale, lse=lse)
     if at is None:
         _call("fck_fmha_fwd", _ptr(q), _ptr(k), _ptr(v), None, _ptr(o), _ptr(cu_seqlens_q), _ptr(cu_seqlens_k), _ptr(seqlen_k), B, tq,
               k.shape[0], Hq, Hk, D, Dv, max_seqlen_q, _scale(scale, D), wl, wr, mask_type, _dtype_id(q), _stream())
@@ -456,8 +465,9 @@ def fmha_fwd_splitkv_fused(q, k, v, num_splits: int = 0, *, seqlen_k=None, block
     return o
 
 
-def fmha_fwd_splitkv_combine(lse_acc, o_acc, dtype, cu_seqlens_q=None, max_seqlen_q: int = 0, out=None) -> torch.Tensor:
-    """LSE combine of split-KV partials -> o [B,sq,Hq,Dv] (or [total_q,Hq,Dv] in group mode)."""
+def fmha_fwd_splitkv_combine(lse_acc, o_acc, dtype, cu_seqlens_q=None, max_seqlen_q: int = 0, out=None, lse=None) -> torch.Tensor:
+    """LSE combine of split-KV partials -> o [B,sq,Hq,Dv] (or [total_q,Hq,Dv] in group mode).  lse (fp32 [B,Hq,sq] or
+    [Hq,total_q], optional) receives the merged log-sum-exp of every row."""
     if dtype not in _DTYPE_ID:
         raise TypeError(f"FMHA supports torch.float16, torch.bfloat16 and torch.float8_e4m3fn, got {dtype}")
     _check_tensor("lse_acc", lse_acc, dtype=torch.float32, ndim=4)
@@ -476,8 +486,14 @@ def fmha_fwd_splitkv_combine(lse_acc, o_acc, dtype, cu_seqlens_q=None, max_seqle
     else:
         B = bs
         o = _out("out", out, (bs, sq, Hq, Dv), dtype, o_acc)
-    _call("fck_fmha_fwd_splitkv_combine", _ptr(lse_acc), _ptr(o_acc), _ptr(o), _ptr(cu_seqlens_q), B, sq, Hq, Dv,
-          max_seqlen_q or sq, ns, _DTYPE_ID[dtype], _stream())
+    if lse is None:
+        _call("fck_fmha_fwd_splitkv_combine", _ptr(lse_acc), _ptr(o_acc), _ptr(o), _ptr(cu_seqlens_q), B, sq, Hq, Dv,
+              max_seqlen_q or sq, ns, _DTYPE_ID[dtype], _stream())
+    else:
+        _check_tensor("lse", lse, dtype=torch.float32)
+        _check_shape("lse", lse, (Hq, sq) if cu_seqlens_q is not None else (bs, Hq, sq), o_acc)
+        _call("fck_fmha_fwd_splitkv_combine_lse", _ptr(lse_acc), _ptr(o_acc), _ptr(o), _ptr(lse), _ptr(cu_seqlens_q), B, sq, Hq, Dv,
+              max_seqlen_q or sq, ns, _DTYPE_ID[dtype], _stream())
     return o
 
 
@@ -585,7 +601,7 @@ def tune_prefill_variant(q, k_cache, v_cache, cu_seqlens_q, kv_indptr, kv_page_i
 def fmha_batch_prefill(q, k_cache, v_cache, cu_seqlens_q, kv_indptr, kv_page_indices, kv_last_page_lens=None, *,
                        max_seqlen_q: int, scale: float = 0.0, mask_type: int = MASK_BOTTOM_RIGHT, window=(-1, 0),
                        out=None, bias=None, alibi_slopes=None, logits_soft_cap: float = 0.0, k_descale: float = 1.0,
-                       v_descale: float = 1.0, prefill_variant: int = 0, o_scale: float = 1.0) -> torch.Tensor:
+                       v_descale: float = 1.0, prefill_variant: int = 0, o_scale: float = 1.0, lse=None) -> torch.Tensor:
     """Varlen prefill over a page list: q [total_q,Hq,D]; sequence b owns pages
     kv_page_indices[kv_indptr[b]:kv_indptr[b+1]] of the cache [num_pages, page_size, Hk, D].  The caches may be
     torch.float8_e4m3fn with the static scales k_descale / v_descale (value = descale * stored); with float8_e4m3fn
@@ -614,7 +630,7 @@ def fmha_batch_prefill(q, k_cache, v_cache, cu_seqlens_q, kv_indptr, kv_page_ind
         prefill_variant = _usable_prefill_variant(tuning.choose_prefill_variant(tuning.prefill_problem(
             Hq, Hk, D, max_seqlen_q, tq, page, "fp16" if q.dtype == torch.float16 else "bf16", mask_type)), D, Dv, max_seqlen_q, page)
     at, keep = _attrs(q, bias, alibi_slopes, logits_soft_cap, True, B, tq, 1, kv_fp8, k_descale, v_descale,
-                      prefill_variant=prefill_variant, o_scale=o_scale)
+                      prefill_variant=prefill_variant, o_scale=o_scale, lse=lse)
     if at is None:
         _call("fck_fmha_batch_prefill", _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(o), _ptr(cu_seqlens_q), _ptr(kv_indptr),
               _ptr(kv_page_indices), _ptr(kv_last_page_lens), num_pages, page, B, Hq, Hk, D, Dv, max_seqlen_q,
@@ -630,7 +646,7 @@ def fmha_batch_prefill(q, k_cache, v_cache, cu_seqlens_q, kv_indptr, kv_page_ind
 def fmha_fwd_pagedkv(q, k_cache, v_cache, seqlen_k, block_table, *, cu_seqlens_q=None, max_seqlen_q: int = 0,
                      scale: float = 0.0, mask_type: int = MASK_BOTTOM_RIGHT, window=(-1, 0), out=None, bias=None,
                      alibi_slopes=None, logits_soft_cap: float = 0.0, k_descale: float = 1.0, v_descale: float = 1.0,
-                     prefill_variant: int = 0, o_scale: float = 1.0) -> torch.Tensor:
+                     prefill_variant: int = 0, o_scale: float = 1.0, lse=None) -> torch.Tensor:
     """Prefill over a block table (no splits): q [B,sq,Hq,D] or packed [total_q,Hq,D].  The caches may be
     torch.float8_e4m3fn with the static scales k_descale / v_descale (value = descale * stored); float8_e4m3fn queries
     and o_scale: see fmha_batch_prefill."""
@@ -657,7 +673,7 @@ def fmha_fwd_pagedkv(q, k_cache, v_cache, seqlen_k, block_table, *, cu_seqlens_q
     wl, wr = _window(window)
     _debug_validate(seqlen_k=seqlen_k, block_table=block_table, num_total_pages=k_cache.shape[0], page_size=page)
     at, keep = _attrs(q, bias, alibi_slopes, logits_soft_cap, group, B, q.shape[0] if group else sq, 1, kv_fp8, k_descale, v_descale,
-                      prefill_variant=prefill_variant, o_scale=o_scale)
+                      prefill_variant=prefill_variant, o_scale=o_scale, lse=lse)
     if at is None:
         _call("fck_fmha_fwd_pagedkv", _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(o), _ptr(cu_seqlens_q), _ptr(seqlen_k),
               _ptr(block_table), block_table.shape[1], page, B, sq, Hq, Hk, D, Dv, max_seqlen_q or sq, _scale(scale, D), wl, wr,
@@ -701,10 +717,11 @@ def fmha_decode_paged(q, k_cache, v_cache, seqlen_k, block_table, *, num_splits:
                       cu_seqlens_q=None, max_seqlen_q: int = 0, scale: float = 0.0, mask_type: int = MASK_NONE,
                       window=(-1, -1), workspace=None, out=None, fused: bool = False, bias=None, alibi_slopes=None,
                       logits_soft_cap: float = 0.0, k_descale: float = 1.0, v_descale: float = 1.0,
-                      decode_variant: int = 0) -> torch.Tensor:
+                      decode_variant: int = 0, lse=None) -> torch.Tensor:
     """Paged decode = split-KV forward + LSE combine; num_splits = 0 asks the tuning cache, then the heuristic (needs
     max_seqlen_k); a cached record also brings the kernel variant it was measured with.  bias / alibi_slopes /
-    logits_soft_cap / fp8 caches with k_descale, v_descale: as fmha_fwd_splitkv (not with fused = True).
+    logits_soft_cap / fp8 caches with k_descale, v_descale: as fmha_fwd_splitkv (not with fused = True).  lse: see
+    fmha_fwd_splitkv_combine (not with fused = True either).
 
     fused = True runs both in one launch that allocates nothing (fmha_fwd_splitkv_fused; the partial results then live
     in the library's fixed device array, `workspace` is not used, and problems beyond its limits raise)."""
@@ -732,8 +749,8 @@ def fmha_decode_paged(q, k_cache, v_cache, seqlen_k, block_table, *, num_splits:
         if not decode_variant:
             decode_variant = _usable_variant(cached_variant, Hq, Hk, sq, D, v_cache.shape[3], plain, k_cache.shape[1])
     if fused:
-        if not plain or decode_variant:
-            raise NotImplementedError("the fused launch takes no bias / soft cap / fp8 cache / kernel variant")
+        if not plain or decode_variant or lse is not None:
+            raise NotImplementedError("the fused launch takes no bias / soft cap / fp8 cache / kernel variant / lse")
         return fmha_fwd_splitkv_fused(q, k_cache, v_cache, num_splits, seqlen_k=seqlen_k, block_table=block_table,
                                       cu_seqlens_q=cu_seqlens_q, max_seqlen_q=max_seqlen_q, scale=scale,
                                       mask_type=mask_type, window=window, out=out)
@@ -743,7 +760,7 @@ def fmha_decode_paged(q, k_cache, v_cache, seqlen_k, block_table, *, num_splits:
                                       mask_type=mask_type, window=window, o_acc=o_acc, lse_acc=lse_acc, bias=bias,
                                       alibi_slopes=alibi_slopes, logits_soft_cap=logits_soft_cap, k_descale=k_descale,
                                       v_descale=v_descale, decode_variant=decode_variant, max_seqlen_k=max_seqlen_k)
-    return fmha_fwd_splitkv_combine(lse_acc, o_acc, q.dtype, cu_seqlens_q=cu_seqlens_q, max_seqlen_q=max_seqlen_q, out=out)
+    return fmha_fwd_splitkv_combine(lse_acc, o_acc, q.dtype, cu_seqlens_q=cu_seqlens_q, max_seqlen_q=max_seqlen_q, out=out, lse=lse)
 
 
 def tune_decode_num_splits(q, k_cache, v_cache, seqlen_k, block_table, *, max_seqlen_k: int,
@@ -873,6 +890,254 @@ def fmha_decode_step(q, knew, vnew, k_cache, v_cache, seqlen_k, block_table, *, 
     return o, seqlen_new
 
 
+def shared_prefix_splits(batch, num_groups, max_group_size, q_num_heads, kv_num_heads, seqlen_q, max_prefix_len, max_own_len,
+                         num_cu=0) -> Tuple[int, int]:
+    """(prefix splits, own splits) fmha_decode_shared_prefix takes by default, from the CU count and the key counts."""
+    ns = (ctypes.c_int32(), ctypes.c_int32())
+    _call("fck_fmha_shared_prefix_splits", batch, num_groups, max_group_size, q_num_heads, kv_num_heads, seqlen_q, max_prefix_len,
+          max_own_len, num_cu, ctypes.byref(ns[0]), ctypes.byref(ns[1]))
+    return ns[0].value, ns[1].value
+
+
+def _check_same_device(like, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != like.device:
+            raise ValueError(f"{name} is on {t.device}, the inputs are on {like.device}")
+
+
+def _on(t):
+    """The device of t made current for a launch (the C ABI launches on the current device and its current stream)."""
+    return torch.cuda.device(t.device) if t.is_cuda else contextlib.nullcontext()
+
+
+def _cache_dtype(q, cache):
+    """(element type a cache next to q must have, whether it is the quantised one)"""
+    kv_fp8 = isinstance(cache, torch.Tensor) and cache.dtype == torch.float8_e4m3fn
+    return (torch.float8_e4m3fn if kv_fp8 else q.dtype), kv_fp8
+
+
+def _check_queries(q, cu_seqlens_q, max_seqlen_q, batch):
+    """(group mode, rows of a head, most query tokens of a sequence) of a query tensor"""
+    group = cu_seqlens_q is not None
+    _check_tensor("q", q, ndim=3 if group else 4)
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"q must be torch.float16 or torch.bfloat16, got {q.dtype}")
+    if q.numel() == 0:
+        raise ValueError("Input tensor cannot be empty")
+    _check_tensor("cu_seqlens_q", cu_seqlens_q, dtype=torch.int32, ndim=1, optional=True)
+    if (cu_seqlens_q.numel() - 1 if group else q.shape[0]) != batch:
+        raise ValueError("seqlen_k must have one entry per sequence of q")
+    if group and max_seqlen_q <= 0:
+        raise ValueError("group mode needs max_seqlen_q")
+    return group, (q.shape[0] if group else q.shape[1]), (int(max_seqlen_q) if group else q.shape[1])
+
+
+def fmha_decode_shared_prefix(q, k_cache, v_cache, seqlen_k, block_table, prefix_lens, *, cu_groups=None, max_group_size: int = 0,
+                              max_prefix_len: int = 0, max_seqlen_k: int = 0, num_prefix_splits: int = 0, num_splits: int = 0,
+                              cu_seqlens_q=None, max_seqlen_q: int = 0, scale: float = 0.0, mask_type: int = MASK_NONE,
+                              window=(-1, -1), alibi_slopes=None, logits_soft_cap: float = 0.0, k_descale: float = 1.0,
+                              v_descale: float = 1.0, workspace: Optional["DecodeWorkspace"] = None, out=None,
+                              lse=None) -> torch.Tensor:
+    """Paged decode attention of a batch whose sequences share prefixes: the result of fmha_decode_paged on the same tensors,
+    with every shared prefix read once per group instead of once per sequence.
+
+    Group g holds the sequences cu_groups[g] .. cu_groups[g+1] - 1 (int32 [G+1], non-decreasing; None: one group, the whole
+    batch) and its sequences have their first prefix_lens[g] tokens (int32 [G], any count) in common.  They are read through
+    the block-table row of the group's first sequence; seqlen_k counts them like all other tokens.
+    Host-side bounds, all optional: max_group_size (sequences of a group beyond it read their own keys), max_prefix_len and
+    max_seqlen_k (they only steer the split counts num_prefix_splits / num_splits, 0 = chosen from them and the CU count).
+    q, masks, windows, ALiBi, soft cap and quantised caches as fmha_decode_paged; no elementwise bias.  workspace keeps the
+    partial results between steps; lse (fp32 [B,Hq,sq] or [Hq,total_q], optional) receives the log-sum-exp of every row."""
+    _check_tensor("seqlen_k", seqlen_k, dtype=torch.int32, ndim=1)
+    B = seqlen_k.numel()
+    group, sq, sq_max = _check_queries(q, cu_seqlens_q, max_seqlen_q, B)
+    cache_dtype, kv_fp8 = _cache_dtype(q, k_cache)
+    _check_tensor("k_cache", k_cache, dtype=cache_dtype, ndim=4)
+    _check_tensor("v_cache", v_cache, dtype=cache_dtype, ndim=4)
+    _check_tensor("block_table", block_table, dtype=torch.int32, ndim=2)
+    _check_tensor("prefix_lens", prefix_lens, dtype=torch.int32, ndim=1)
+    _check_tensor("cu_groups", cu_groups, dtype=torch.int32, ndim=1, optional=True)
+    _check_kv(q, k_cache, v_cache, 4)
+    if block_table.shape[0] != B:
+        raise ValueError(f"block_table must be [batch, max_pages_per_seq] with batch {B}, got {tuple(block_table.shape)}")
+    G = prefix_lens.numel()
+    if G < 1 or (G != 1 if cu_groups is None else cu_groups.numel() != G + 1):
+        raise ValueError(f"prefix_lens must have one entry per group ({G}), cu_groups one more"
+                         f" ({None if cu_groups is None else cu_groups.numel()}; without it there is one group)")
+    _check_same_device(q, k_cache=k_cache, v_cache=v_cache, seqlen_k=seqlen_k, block_table=block_table, prefix_lens=prefix_lens,
+                       cu_groups=cu_groups, cu_seqlens_q=cu_seqlens_q, alibi_slopes=alibi_slopes)
+    Hq, D = q.shape[-2], q.shape[-1]
+    page, Hk, Dv = k_cache.shape[1], k_cache.shape[2], v_cache.shape[3]
+    capacity = block_table.shape[1] * page
+    if capacity == 0:
+        raise ValueError("block_table must have at least one page per sequence")
+    max_group_size = min(int(max_group_size), B) if max_group_size > 0 else B
+    if num_prefix_splits <= 0 or num_splits <= 0:
+        longest = max_seqlen_k if max_seqlen_k > 0 else capacity
+        prefix = min(max_prefix_len, longest) if max_prefix_len > 0 else longest
+        ns = shared_prefix_splits(B, G, max_group_size, Hq, Hk, sq_max, prefix, longest - prefix if max_prefix_len > 0 else longest)
+        num_prefix_splits = num_prefix_splits if num_prefix_splits > 0 else ns[0]
+        num_splits = num_splits if num_splits > 0 else ns[1]
+    _debug_validate(seqlen_k=seqlen_k, block_table=block_table, num_total_pages=k_cache.shape[0], page_size=page)
+    o = _out("out", out, (*q.shape[:-1], Dv), q.dtype, q)
+    if lse is not None:
+        _check_tensor("lse", lse, dtype=torch.float32)
+        _check_shape("lse", lse, (Hq, sq) if group else (B, Hq, sq), q)
+    shape_batch, total = (1 if group else B), int(num_prefix_splits) + int(num_splits)
+    if workspace is not None:
+        o_acc, lse_acc = workspace.partials(shape_batch, Hq, total, sq, Dv, q.device)
+    else:
+        o_acc, lse_acc = splitkv_workspace(shape_batch, Hq, sq, Dv, total, q.device)
+    wl, wr = _window(window)
+    at, keep = _attrs(q, None, alibi_slopes, logits_soft_cap, group, B, sq, 1, kv_fp8, k_descale, v_descale)
+    with _on(q):
+        _call("fck_fmha_decode_shared_prefix", _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(o), _ptr(lse), _ptr(lse_acc), _ptr(o_acc),
+              _ptr(cu_seqlens_q), _ptr(seqlen_k), _ptr(block_table), _ptr(cu_groups), _ptr(prefix_lens), B, G, max_group_size, sq, Hq,
+              Hk, D, Dv, sq_max, int(num_prefix_splits), int(num_splits), block_table.shape[1], page, _scale(scale, D), wl, wr,
+              mask_type, _dtype_id(q), at, _stream())
+    del keep
+    return o
+
+
+def fmha_key_weights(q, k_cache, lse, seqlen_k, block_table=None, *, weights=None, cu_seqlens_q=None, max_seqlen_q: int = 0,
+                     max_seqlen_k: int = 0, scale: float = 0.0, mask_type: int = MASK_NONE, window=(-1, -1), alibi_slopes=None,
+                     logits_soft_cap: float = 0.0, k_descale: float = 1.0, out=None) -> torch.Tensor:
+    """Attention weight every cached key receives, fp32 [B, Hk, cols]:
+
+        out[b, hk, t] = weights[b, hk, t] + sum over the query heads h of KV head hk and the rows i that see t of
+                        exp(score(b, h, i, t) - lse[b, h, i])
+
+    lse (fp32 [B,Hq,sq], packed queries [Hq,total_q]) is what the attention over the same keys returned (lse= of fmha_fwd,
+    fmha_batch_prefill, fmha_fwd_pagedkv, fmha_decode_paged, fmha_decode_shared_prefix); rows with -inf add nothing.
+    k_cache is a paged cache with block_table, or [B, sk, Hk, D] without one (seqlen_k may then be None).
+    weights (optional) are what earlier steps accumulated; out may be the same tensor.  cols is their last dimension, else
+    max_seqlen_k, else what the cache can hold.  Entries at and behind a sequence's key count are written as 0, so the tensor
+    can go on growing with its cache.  Masks, windows, ALiBi, soft cap and quantised keys as the attention operators."""
+    if seqlen_k is None and block_table is not None:
+        raise ValueError("a paged cache needs seqlen_k")
+    _check_tensor("seqlen_k", seqlen_k, dtype=torch.int32, ndim=1, optional=True)
+    if not isinstance(k_cache, torch.Tensor):
+        raise TypeError(f"Expected k_cache to be a torch.Tensor, got {type(k_cache)}")
+    B = seqlen_k.numel() if seqlen_k is not None else k_cache.shape[0]
+    group, sq, sq_max = _check_queries(q, cu_seqlens_q, max_seqlen_q, B)
+    cache_dtype, kv_fp8 = _cache_dtype(q, k_cache)
+    _check_tensor("k_cache", k_cache, dtype=cache_dtype, ndim=4)
+    _check_tensor("block_table", block_table, dtype=torch.int32, ndim=2, optional=True)
+    _check_kv(q, k_cache, k_cache, 3 if k_cache.dim() == 3 else 4)
+    Hq, D, Hk = q.shape[-2], q.shape[-1], k_cache.shape[2]
+    if block_table is not None:
+        if block_table.shape[0] != B:
+            raise ValueError(f"block_table must be [batch, max_pages_per_seq] with batch {B}, got {tuple(block_table.shape)}")
+        stride, page, sk = block_table.shape[1], k_cache.shape[1], 0
+        capacity = stride * page
+    else:
+        if k_cache.shape[0] != B:
+            raise ValueError(f"k_cache {tuple(k_cache.shape)} must have one row per sequence ({B}) without a block table")
+        stride, page, sk = 0, 0, k_cache.shape[1]
+        capacity = sk
+    _check_tensor("lse", lse, dtype=torch.float32)
+    _check_shape("lse", lse, (Hq, sq) if group else (B, Hq, sq), q)
+    _check_tensor("weights", weights, dtype=torch.float32, ndim=3, optional=True)
+    _check_tensor("out", out, dtype=torch.float32, ndim=3, optional=True)
+    given = weights if weights is not None else out
+    cols = given.shape[2] if given is not None else max_seqlen_k if max_seqlen_k > 0 else capacity
+    if cols <= 0 or capacity <= 0:
+        raise ValueError("the cache and the weights need at least one key per sequence")
+    if weights is not None:
+        _check_shape("weights", weights, (B, Hk, cols), q)
+    _check_same_device(q, k_cache=k_cache, seqlen_k=seqlen_k, block_table=block_table, cu_seqlens_q=cu_seqlens_q,
+                       alibi_slopes=alibi_slopes)
+    if block_table is not None:
+        _debug_validate(seqlen_k=seqlen_k, block_table=block_table, num_total_pages=k_cache.shape[0], page_size=page)
+    o = _out("out", out, (B, Hk, cols), torch.float32, q)
+    wl, wr = _window(window)
+    at, keep = _attrs(q, None, alibi_slopes, logits_soft_cap, group, B, sq, 1, kv_fp8, k_descale, 1.0)
+    with _on(q):
+        _call("fck_fmha_key_weights", _ptr(q), _ptr(k_cache), _ptr(lse), _ptr(weights), _ptr(o), _ptr(cu_seqlens_q), _ptr(seqlen_k),
+              _ptr(block_table), stride, page, B, sq, sk, cols, Hq, Hk, D, sq_max, _scale(scale, D), wl, wr, mask_type, _dtype_id(q),
+              at, _stream())
+    del keep
+    return o
+
+
+def fmha_cache_evict(k_cache, v_cache, weights, seqlen_k, block_table, new_block_table, *, budget: int, recent: int = 0,
+                     sinks: int = 0, new_k_cache=None, new_v_cache=None, out_seqlen=None, out_kept=None, out_weights=None):
+    """Keep at most `budget` keys of every (sequence, KV head) of a paged cache and move their rows to new pages.
+
+    A sequence of L keys keeps n = min(L, budget): all of them when L <= budget, else its first `sinks`, its last `recent` and,
+    of the keys between, those with the largest weights (weights fp32 [B, Hk, cols] as fmha_key_weights accumulates them;
+    equal weights: the lower position; NaN counts as -inf).  Slot j of sequence b in the pages of new_block_table (int32
+    [B, pages], at least `budget` keys a row) receives, for each head, the row of its j-th kept key in ascending order.
+    The rows go to new_k_cache / new_v_cache (default: the same pools); pages that block_table names are never written, as other
+    sequences may share them, so new_block_table must name other pages then.  After the call the old pages can be reused.
+    Heads keep different positions: masks that go by position do not apply to evicted keys any more.
+
+    Returns (seqlen_k_new int32 [B], kept int32 [B, Hk, budget] with -1 behind the n-th, weights_new fp32 [B, Hk, cols] with
+    zeros behind the n-th)."""
+    _check_tensor("k_cache", k_cache, ndim=4)
+    _dtype_id(k_cache)
+    _check_tensor("v_cache", v_cache, dtype=k_cache.dtype, ndim=4)
+    _check_tensor("new_k_cache", new_k_cache, dtype=k_cache.dtype, ndim=4, optional=True)
+    _check_tensor("new_v_cache", new_v_cache, dtype=k_cache.dtype, ndim=4, optional=True)
+    if (new_k_cache is None) != (new_v_cache is None):
+        raise ValueError("new_k_cache and new_v_cache must be given together")
+    nk, nv = (k_cache, v_cache) if new_k_cache is None else (new_k_cache, new_v_cache)
+    if v_cache.shape[:3] != k_cache.shape[:3]:
+        raise ValueError(f"v_cache {tuple(v_cache.shape)} does not match k_cache {tuple(k_cache.shape)}")
+    if nk.shape[2:] != k_cache.shape[2:] or nv.shape[2:] != v_cache.shape[2:] or nk.shape[:2] != nv.shape[:2]:
+        raise ValueError(f"new_k_cache {tuple(nk.shape)} / new_v_cache {tuple(nv.shape)} do not match k_cache {tuple(k_cache.shape)} / "
+                         f"v_cache {tuple(v_cache.shape)}")
+    _, page, Hk, D = k_cache.shape
+    _check_tensor("seqlen_k", seqlen_k, dtype=torch.int32, ndim=1)
+    _check_tensor("block_table", block_table, dtype=torch.int32, ndim=2)
+    _check_tensor("new_block_table", new_block_table, dtype=torch.int32, ndim=2)
+    B = seqlen_k.numel()
+    if B == 0 or block_table.shape[0] != B or new_block_table.shape[0] != B or block_table.shape[1] == 0:
+        raise ValueError(f"block_table {tuple(block_table.shape)} and new_block_table {tuple(new_block_table.shape)} must have one row per "
+                         f"sequence ({B})")
+    _check_tensor("weights", weights, dtype=torch.float32, ndim=3)
+    cols = weights.shape[2]
+    _check_shape("weights", weights, (B, Hk, cols), k_cache)
+    budget, recent, sinks = int(budget), int(recent), int(sinks)
+    if budget <= 0 or recent < 0 or sinks < 0 or recent + sinks > budget:
+        raise ValueError(f"budget {budget} must be positive and hold recent {recent} + sinks {sinks}")
+    if new_block_table.shape[1] * nk.shape[1] < budget:
+        raise ValueError(f"a row of new_block_table addresses {new_block_table.shape[1] * nk.shape[1]} keys, the budget is {budget}")
+    same_pool = nk.data_ptr() == k_cache.data_ptr() or nv.data_ptr() == v_cache.data_ptr()
+    if same_pool and new_block_table.data_ptr() == block_table.data_ptr():
+        raise ValueError("new_block_table must name other pages than block_table: rows are not moved inside the pages that are read")
+    _check_same_device(k_cache, v_cache=v_cache, new_k_cache=nk, new_v_cache=nv, seqlen_k=seqlen_k, block_table=block_table,
+                       new_block_table=new_block_table)
+    seqlen_new = _out("out_seqlen", out_seqlen, (B,), torch.int32, k_cache)
+    kept = _out("out_kept", out_kept, (B, Hk, budget), torch.int32, k_cache)
+    weights_new = _out("out_weights", out_weights, (B, Hk, cols), torch.float32, k_cache)
+    if weights_new.data_ptr() == weights.data_ptr():
+        raise ValueError("out_weights must not be weights")
+    if seqlen_new.data_ptr() == seqlen_k.data_ptr():
+        raise ValueError("out_seqlen must not be seqlen_k")
+    if flags.flag("FC_DEBUG_KERNEL_INSTANCE"):
+        validate_paged(seqlen_k=seqlen_k, block_table=block_table, num_total_pages=k_cache.shape[0], page_size=page, check=True)
+        _validate_new_pages(seqlen_k, block_table, new_block_table, budget, page, nk, same_pool)
+    with _on(k_cache):
+        _call("fck_fmha_cache_evict", _ptr(k_cache), _ptr(v_cache), _ptr(nk), _ptr(nv), _ptr(weights), _ptr(weights_new), _ptr(seqlen_k),
+              _ptr(seqlen_new), _ptr(kept), _ptr(block_table), block_table.shape[1], page, _ptr(new_block_table), new_block_table.shape[1],
+              nk.shape[1], B, Hk, D, v_cache.shape[3], cols, budget, recent, sinks, _dtype_id(k_cache), _stream())
+    return seqlen_new, kept, weights_new
+
+
+def _validate_new_pages(seqlen_k, block_table, new_block_table, budget, page, new_cache, same_pool):
+    """The pages an eviction writes: inside the pool, each used once, and none of those it reads (debug aid; synchronises)."""
+    new_page = new_cache.shape[1]
+    lens, old, new = seqlen_k.tolist(), block_table.tolist(), new_block_table.tolist()
+    written = [p for n, row in zip(lens, new) for p in row[:-(-min(n, budget) // new_page)]]
+    if any(p < 0 or p >= new_cache.shape[0] for p in written):
+        raise ValueError(f"new_block_table names a page outside the pool of {new_cache.shape[0]}")
+    if len(set(written)) != len(written):
+        raise ValueError("new_block_table names a page twice")
+    if same_pool and set(written) & {p for n, row in zip(lens, old) for p in row[:-(-n // page)]}:
+        raise ValueError("new_block_table names a page that block_table reads")
+
+
 register_flashck_functions(FlashCKOperationType.FMHA.value, {
     "forward": fmha_fwd,
     "forward_varlen": fmha_fwd_varlen,
@@ -883,4 +1148,7 @@ register_flashck_functions(FlashCKOperationType.FMHA.value, {
     "forward_pagedkv": fmha_fwd_pagedkv,
     "decode_paged": fmha_decode_paged,
     "decode_step": fmha_decode_step,
+    "decode_shared_prefix": fmha_decode_shared_prefix,
+    "key_weights": fmha_key_weights,
+    "cache_evict": fmha_cache_evict,
 })

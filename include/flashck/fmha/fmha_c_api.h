@@ -127,6 +127,12 @@ typedef struct fck_fmha_attrs {
     /* dtype FCK_DTYPE_FP8 on fck_fmha_fwd / _pagedkv / _batch_prefill: the output is saturate(o_scale * o) in e4m3
      * (ck_tile's scale_o; the reference passes 1).  0 means 1.  The split-KV pair writes with scale 1. */
     float o_scale;
+    /* fck_fmha_fwd / _pagedkv / _batch_prefill: when not NULL, the log-sum-exp of every row's scores (natural log; -inf for a
+     * row that sees no key) as fp32 in caller-owned device memory: batch mode (b, h, i) at ((b * q_num_heads) + h) *
+     * lse_head_stride + i, group mode (h, packed row) at h * lse_head_stride + row.  A caller built against the struct
+     * without these two fields (its `size` says so) is served as before. */
+    float* lse;
+    int64_t lse_head_stride;
 } fck_fmha_attrs;
 
 #define FCK_OK 0
@@ -266,6 +272,91 @@ FCK_EXPORT int fck_fmha_fwd_splitkv_combine(const void* lse_acc, const void* o_a
                                             const int32_t* seqstart_q, int64_t batch, int64_t seqlen_q,
                                             int64_t q_num_heads, int64_t v_head_dim, int64_t q_max_seq_len,
                                             int64_t num_splits, int32_t dtype, void* stream);
+
+/* The same, and the merged log-sum-exp of every row as fp32 in lse ([B, Hq, sq], group mode [Hq, total_q]; NULL: not
+ * written). */
+FCK_EXPORT int fck_fmha_fwd_splitkv_combine_lse(const void* lse_acc, const void* o_acc, void* o, void* lse,
+                                                const int32_t* seqstart_q, int64_t batch, int64_t seqlen_q,
+                                                int64_t q_num_heads, int64_t v_head_dim, int64_t q_max_seq_len,
+                                                int64_t num_splits, int32_t dtype, void* stream);
+
+/*
+ * Decode attention over a paged cache for a batch whose sequences share prefixes: what fck_fmha_fwd_splitkv + _combine
+ * compute over the same block table, with every shared prefix read once per group instead of once per sequence.
+ *   groups        group g holds the sequences [cu_groups[g], cu_groups[g+1]) (int32 [num_groups + 1], non-decreasing,
+ *                 inside [0, batch]; NULL: one group, the whole batch); sequences of no group share nothing
+ *   prefix_lens   int32 [num_groups]: tokens the group's sequences have in common, from their first on (any count; clamped
+ *                 to what the group's first sequence has).  They are read through the first sequence's block-table row, so
+ *                 the rows of the others need not be set up for whole pages of them.
+ *   max_group_size  at most this many sequences of a group share (0: batch); the ones behind read all their own keys
+ *   seqlen_k_ptr  int32 [B], key counts with the prefix
+ *   q, o, lse     as fck_fmha_fwd_splitkv and its combine; seqlen_q carries total_q in group mode; lse may be NULL
+ *   o_acc, lse_acc  fp32 workspace [Bs, Hq, num_prefix_splits + num_own_splits, Sq, Dv] and without Dv
+ *                 (fck_fmha_splitkv_workspace_bytes); split counts in [1, 64], fck_fmha_shared_prefix_splits chooses them
+ * attrs: ALiBi, soft cap, kv_dtype with its scales.  Two launches.  A row whose mask leaves no key gets zeros and lse -inf;
+ * rows behind the last sequence of packed queries are left as they were.  No counterpart in the reference.
+ */
+FCK_EXPORT int fck_fmha_decode_shared_prefix(const void* q, const void* k_cache, const void* v_cache, void* o, void* lse,
+                                             void* lse_acc, void* o_acc, const int32_t* seqstart_q,
+                                             const int32_t* seqlen_k_ptr, const int32_t* block_table,
+                                             const int32_t* cu_groups, const int32_t* prefix_lens, int64_t batch,
+                                             int64_t num_groups, int64_t max_group_size, int64_t seqlen_q,
+                                             int64_t q_num_heads, int64_t kv_num_heads, int64_t qk_head_dim,
+                                             int64_t v_head_dim, int64_t q_max_seq_len, int64_t num_prefix_splits,
+                                             int64_t num_own_splits, int64_t batch_stride_block_table,
+                                             int64_t page_block_size, float scale, int64_t window_left,
+                                             int64_t window_right, uint32_t mask_type, int32_t dtype,
+                                             const fck_fmha_attrs* attrs, void* stream);
+
+/* Split counts for fck_fmha_decode_shared_prefix from the CU count (num_cu <= 0: of the current device) and the longest
+ * prefix and the most keys a sequence has behind it. */
+FCK_EXPORT int fck_fmha_shared_prefix_splits(int64_t batch, int64_t num_groups, int64_t max_group_size, int64_t q_num_heads,
+                                             int64_t kv_num_heads, int64_t seqlen_q, int64_t max_prefix_len,
+                                             int64_t max_own_len, int64_t num_cu, int32_t* prefix_splits,
+                                             int32_t* own_splits);
+
+/*
+ * Attention weight every key receives:
+ *   out[b, hk, t] = weights[b, hk, t] + sum over the query heads h of KV head hk and the rows i that see key t of
+ *                   exp(s - lse[b, h, i]),  s the score of (b, h, i, t) as the attention entry points define it
+ *   lse      fp32 [B, Hq, sq] (group mode [Hq, total_q]): the log-sum-exp the attention over the same keys returned
+ *            (fck_fmha_attrs.lse, _combine_lse, fck_fmha_decode_shared_prefix); a row with -inf adds nothing
+ *   weights, out  fp32 [B, Hk, cols]; weights may be NULL (zeros) or out itself.  Entries at and behind a sequence's key
+ *            count are written as 0; keys at and behind cols have no entry.
+ *   k        paged cache with block_table + seqlen_k_ptr, or (block_table NULL) batch cache [B, seqlen_k, Hk, D] with optional
+ *            seqlen_k_ptr.  seqlen_q carries total_q in group mode.
+ * attrs: ALiBi, soft cap, kv_dtype with k_descale.  No counterpart in the reference.
+ */
+FCK_EXPORT int fck_fmha_key_weights(const void* q, const void* k, const void* lse, const void* weights, void* out,
+                                    const int32_t* seqstart_q, const int32_t* seqlen_k_ptr, const int32_t* block_table,
+                                    int64_t batch_stride_block_table, int64_t page_block_size, int64_t batch,
+                                    int64_t seqlen_q, int64_t seqlen_k, int64_t cols, int64_t q_num_heads,
+                                    int64_t kv_num_heads, int64_t qk_head_dim, int64_t q_max_seq_len, float scale,
+                                    int64_t window_left, int64_t window_right, uint32_t mask_type, int32_t dtype,
+                                    const fck_fmha_attrs* attrs, void* stream);
+
+/*
+ * Eviction: every (sequence, KV head) keeps n = min(seqlen_k[b], budget) keys: all of them when seqlen_k[b] <= budget, else
+ * the first `sinks`, the last `recent` (sinks + recent <= budget) and, of the keys between, those with the largest weights
+ * (ties: the lower position; a NaN counts as -inf; a position at or behind cols counts as weight 0).
+ *   kept          int32 [B, Hk, budget]: the kept positions in ascending order, -1 behind the n-th
+ *   new_seqlen_k  int32 [B]: n
+ *   new_weights   fp32 [B, Hk, cols]: the weights of the kept keys, zeros behind; must not be `weights`
+ *   new_k_cache, new_v_cache, new_block_table (int32 [B, new_batch_stride_block_table], >= budget keys a row): where the kept
+ *                 rows go, slot j of sequence b for the j-th kept key of each head.  The pools may be the ones that are read;
+ *                 the pages must then be other pages than any that block_table names (which may be shared by sequences and
+ *                 are never written).
+ * dtype is the element type of the caches.  The positions of a head's kept keys differ between heads, so masks that go by
+ * position do not apply to the evicted keys.  No counterpart in the reference.
+ */
+FCK_EXPORT int fck_fmha_cache_evict(const void* k_cache, const void* v_cache, void* new_k_cache, void* new_v_cache,
+                                    const void* weights, void* new_weights, const int32_t* seqlen_k,
+                                    int32_t* new_seqlen_k, int32_t* kept, const int32_t* block_table,
+                                    int64_t batch_stride_block_table, int64_t page_block_size,
+                                    const int32_t* new_block_table, int64_t new_batch_stride_block_table,
+                                    int64_t new_page_block_size, int64_t batch, int64_t kv_num_heads, int64_t qk_head_dim,
+                                    int64_t v_head_dim, int64_t cols, int64_t budget, int64_t recent, int64_t sinks,
+                                    int32_t dtype, void* stream);
 
 /*
  * AppendKV: rotate knew (and q, in place) and write knew / vnew behind the seqlen_k[b] tokens each sequence
