@@ -12,7 +12,7 @@ namespace fck {
 namespace {
 
 constexpr int kThreads = 1024;
-constexpr int kSelectWaves = kThreads / 64;
+constexpr int kWaves = kThreads / 64;
 
 // order-preserving map of a weight to an unsigned key; -0 and +0 are equal, NaN is -inf
 __device__ __forceinline__ uint32_t weight_key(float w)
@@ -23,124 +23,241 @@ __device__ __forceinline__ uint32_t weight_key(float w)
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// One workgroup per (sequence, KV head).  The k-th largest key of the middle is found 8 bits at a time from a histogram in
-// LDS; then one ordered pass over the positions writes the kept ones (ranks by ballot and a prefix sum over the waves).
+// One workgroup per (sequence, KV head); bound by the walks over its weights (L2 round trips), so they are few and wide: a wave
+// owns a contiguous sixteenth of the row and reads 4 weights per lane and load.
+//   1. The want-th largest key of the middle, 8 bits per walk, from a histogram in LDS with a column per lane: lanes never
+//      meet at an address or a bank whatever the weights are (a single histogram serialised on the many equal weights, zeros
+//      above all: 369 us for one sequence of 131072 keys and 8 heads).
+//   2. A walk that counts what each wave keeps, and one that writes it from the wave's first rank on: ranks are ballots, and
+//      no barrier lies inside a walk.
 __global__ __launch_bounds__(kThreads) void evict_select_kernel(const CacheEvictArgs a)
 {
-    __shared__ int hist[256];
-    __shared__ int chosen[2];
-    __shared__ int wave_count[2][kSelectWaves];
+    __shared__ int hist[256 * 64];  // [digit][lane]
+    __shared__ __align__(16) int digits[256];
+    __shared__ int chosen[3];
+    __shared__ int counts[2][kWaves];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hkv = blockIdx.x % a.hk, b = blockIdx.x / a.hk;
     const int64_t cap = (int64_t)a.block_table_stride * a.page_size;
-    const int len = (int)min((int64_t)max(a.seqlen_k[b], 0), cap);
+    const int len = __builtin_amdgcn_readfirstlane((int)min((int64_t)max(a.seqlen_k[b], 0), cap));
     const int n_keep = min(len, a.budget);
-    const float* w = a.weights + ((int64_t)b * a.hk + hkv) * a.cols;
-    float* nw = a.new_weights + ((int64_t)b * a.hk + hkv) * a.cols;
-    int32_t* kept = a.kept + ((int64_t)b * a.hk + hkv) * a.budget;
-    // a position the weights have no column for has received nothing
-    auto weight = [&](int t) { return t < a.cols ? w[t] : 0.f; };
+    const float* const w = a.weights + ((int64_t)b * a.hk + hkv) * a.cols;
+    float* const nw = a.new_weights + ((int64_t)b * a.hk + hkv) * a.cols;
+    int32_t* const kept = a.kept + ((int64_t)b * a.hk + hkv) * a.budget;
+    const bool vec = a.cols % 4 == 0 && (reinterpret_cast<uintptr_t>(a.weights) & 15) == 0;
 
     // positions [0, lo) and [hi, len) are kept anyway, `want` of [lo, hi) by weight
     const bool all = len <= a.budget;
     const int lo = all ? len : a.sinks, hi = all ? len : len - a.recent;
     const int want = all ? 0 : a.budget - a.sinks - a.recent;
-    uint32_t threshold = 0;  // the want-th largest key
+
+    const int seg = ((len + kWaves - 1) / kWaves + 255) / 256 * 256;
+    const int seg0 = (int)min((int64_t)wave * seg, (int64_t)len), seg1 = (int)min((int64_t)(wave + 1) * seg, (int64_t)len);
+    // the 4 weights from position t on; a position the weights have no column for has received nothing
+    auto load4 = [&](int t) -> f32x4_t {
+        if (vec && t + 4 <= a.cols) return *reinterpret_cast<const f32x4_t*>(w + t);
+        f32x4_t x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = t + e < a.cols ? w[t + e] : 0.f;
+        return x;
+    };
+    // calls f(position of the lane's first weight, its 4 weights) for the wave's segment; positions from len on are the
+    // caller's to leave out.  Four loads are in flight per lane.
+    auto walk = [&](auto f) {
+        int t0 = seg0;
+        for (; t0 + 1024 <= seg1; t0 += 1024) {
+            f32x4_t x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] = load4(t0 + u * 256 + lane * 4);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) f(t0 + u * 256 + lane * 4, x[u]);
+        }
+        for (; t0 < seg1; t0 += 256) f(t0 + lane * 4, load4(t0 + lane * 4));
+    };
+
+    uint32_t threshold = 0;  // the want-th largest key, in the digits that decide
     int equal_wanted = 0;    // how many of the positions whose key equals it are kept
     if (want > 0) {
         uint32_t mask = 0;
         int left = want;
         for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
+            for (int e = tid; e < 256 * 64; e += kThreads) hist[e] = 0;
             __syncthreads();
-            for (int t = lo + tid; t < hi; t += kThreads) {
-                const uint32_t key = weight_key(weight(t));
-                if ((key & mask) == threshold) atomicAdd(&hist[key >> shift & 255], 1);
+            walk([&](int t, const f32x4_t& x) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t key = weight_key(x[e]);
+                    if (t + e >= lo && t + e < hi && (key & mask) == threshold) atomicAdd(&hist[(key >> shift & 255) * 64 + lane], 1);
+                }
+            });
+            __syncthreads();
+            if (tid < 256) {
+                int sum = 0;
+                for (int c = 0; c < 64; ++c) sum += hist[tid * 64 + ((c + tid) & 63)];
+                digits[tid] = sum;
             }
             __syncthreads();
-            if (tid == 0) {
-                int digit = 255, above = 0;
-                while (digit > 0 && above + hist[digit] < left) above += hist[digit--];
-                chosen[0] = digit;
-                chosen[1] = left - above;
+            if (tid < 256) {
+                int above = 0;
+                for (int d = 0; d < 256; d += 4) {
+                    const u32x4_t n = *reinterpret_cast<const u32x4_t*>(&digits[d]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) above += d + e > tid ? (int)n[e] : 0;
+                }
+                const int here = digits[tid];
+                if (above < left && left <= above + here) {  // exactly one thread
+                    chosen[0] = tid;
+                    chosen[1] = left - above;
+                    chosen[2] = here;
+                }
             }
             __syncthreads();
             threshold |= (uint32_t)chosen[0] << shift;
             left = chosen[1];
             mask |= 255u << shift;
-            __syncthreads();
+            if (chosen[2] == left) break;  // every key that begins like this is kept: the digits behind do not matter
         }
         equal_wanted = left;
-    }
-
-    int n_before = 0, eq_before = 0;  // kept positions and equal keys ahead of this chunk
-    for (int t0 = 0; t0 < len; t0 += kThreads) {
-        const int t = t0 + tid;
-        const float wt = t < len ? weight(t) : 0.f;
-        const bool middle = t >= lo && t < hi;
-        const uint32_t key = weight_key(wt);
-        const bool equal = middle && want > 0 && key == threshold;
-        const uint64_t eq_mask = __builtin_amdgcn_ballot_w64(equal);
-        const uint64_t below = ((uint64_t)1 << lane) - 1;
-        if (lane == 0) wave_count[0][wave] = __builtin_popcountll(eq_mask);
+        const uint32_t m = mask;
+        int sure = 0, equal = 0;
+        walk([&](int t, const f32x4_t& x) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int p = t + e;
+                const uint32_t key = weight_key(x[e]) & m;
+                const bool middle = p >= lo && p < hi;
+                sure += __builtin_popcountll(__builtin_amdgcn_ballot_w64(p < len && (!middle || key > threshold)));
+                equal += __builtin_popcountll(__builtin_amdgcn_ballot_w64(middle && key == threshold));
+            }
+        });
+        if (lane == 0) {
+            counts[0][wave] = sure;
+            counts[1][wave] = equal;
+        }
         __syncthreads();
-        int eq_rank = eq_before + __builtin_popcountll(eq_mask & below), eq_total = 0;
-        for (int v = 0; v < kSelectWaves; ++v) {
-            if (v < wave) eq_rank += wave_count[0][v];
-            eq_total += wave_count[0][v];
+        int rank = 0, equal_left = equal_wanted;
+        for (int v = 0; v < wave; ++v) {
+            const int eq = min(counts[1][v], equal_left);
+            rank += counts[0][v] + eq;
+            equal_left -= eq;
         }
-        const bool keep = t < len && (!middle || (want > 0 && (key > threshold || (equal && eq_rank < equal_wanted))));
-        const uint64_t keep_mask = __builtin_amdgcn_ballot_w64(keep);
-        if (lane == 0) wave_count[1][wave] = __builtin_popcountll(keep_mask);
-        __syncthreads();
-        int rank = n_before + __builtin_popcountll(keep_mask & below), total = 0;
-        for (int v = 0; v < kSelectWaves; ++v) {
-            if (v < wave) rank += wave_count[1][v];
-            total += wave_count[1][v];
+        walk([&](int t, const f32x4_t& x) {
+            // per element: kept without question, or equal to the threshold and early enough
+            uint64_t keep_mask[4], eq_mask[4];
+            bool mine[4], eq[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int p = t + e;
+                const uint32_t key = weight_key(x[e]) & m;
+                const bool middle = p >= lo && p < hi;
+                mine[e] = p < len && (!middle || key > threshold);
+                eq[e] = middle && key == threshold;
+                eq_mask[e] = __builtin_amdgcn_ballot_w64(eq[e]);
+            }
+            const uint64_t below = ((uint64_t)1 << lane) - 1;
+            int eq_rank = 0, eq_total = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                eq_rank += __builtin_popcountll(eq_mask[e] & below);
+                eq_total += __builtin_popcountll(eq_mask[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (eq[e] && eq_rank < equal_left) mine[e] = true;
+                eq_rank += eq[e] ? 1 : 0;
+            }
+            equal_left = max(equal_left - eq_total, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) keep_mask[e] = __builtin_amdgcn_ballot_w64(mine[e]);
+            int at = rank;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                at += __builtin_popcountll(keep_mask[e] & below);
+                rank += __builtin_popcountll(keep_mask[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (mine[e]) {
+                    if (at < n_keep) {
+                        kept[at] = t + e;
+                        if (at < a.cols) nw[at] = x[e];
+                    }
+                    ++at;
+                }
+        });
+    } else {
+        // all of them, or the sinks and the most recent ones
+        for (int j = tid; j < n_keep; j += kThreads) {
+            const int t = all || j < a.sinks ? j : len - n_keep + j;
+            kept[j] = t;
+            if (j < a.cols) nw[j] = t < a.cols ? w[t] : 0.f;
         }
-        if (keep && rank < n_keep) {
-            kept[rank] = t;
-            if (rank < a.cols) nw[rank] = wt;
-        }
-        n_before += total;
-        eq_before += eq_total;
     }
     for (int j = n_keep + tid; j < a.budget; j += kThreads) kept[j] = -1;
-    for (int64_t j = n_keep + tid; j < a.cols; j += kThreads) nw[j] = 0.f;
+    int64_t z = min(((int64_t)n_keep + 3) / 4 * 4, a.cols);
+    if (n_keep + tid < z) nw[n_keep + tid] = 0.f;
+    if (vec && (reinterpret_cast<uintptr_t>(a.new_weights) & 15) == 0)
+        for (z += tid * 4; z < a.cols; z += kThreads * 4) *reinterpret_cast<f32x4_t*>(nw + z) = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    else
+        for (z += tid; z < a.cols; z += kThreads) nw[z] = 0.f;
     if (hkv == 0 && tid == 0) a.new_seqlen[b] = n_keep;
 }
 
-// Copies the kept rows.  Unit: one 8-byte or 16-byte piece of K or V of one (slot, KV head).
+// Copies the kept rows.  A thread moves one 8- or 16-byte piece of K and of V of one KV head for kSlots consecutive slots, so
+// that the chain position -> page -> row is walked for all of them at once and 2 kSlots loads are in flight; consecutive
+// threads write consecutive pieces of a slot's row.
+constexpr int kSlots = 4;
 template <typename Piece>
 __global__ __launch_bounds__(256) void evict_move_kernel(const CacheEvictArgs a)
 {
-    const int kp = a.k_row / (int)sizeof(Piece), vp = a.v_row / (int)sizeof(Piece);
-    const int per_head = kp + vp;
-    const int64_t item = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int piece = (int)(item % per_head);
-    const int hkv = (int)(item / per_head % a.hk);
-    const int64_t s = item / per_head / a.hk;
-    const int slot = (int)(s % a.budget);
-    const int64_t b = s / a.budget;
+    const uint32_t kp = a.k_row / (uint32_t)sizeof(Piece), vp = a.v_row / (uint32_t)sizeof(Piece);
+    const uint32_t pieces = max(kp, vp), per_seq = (uint32_t)(a.budget + kSlots - 1) / kSlots;
+    uint32_t id = blockIdx.x * 256u + threadIdx.x;
+    const uint32_t piece = id % pieces;
+    id /= pieces;
+    const uint32_t hkv = id % (uint32_t)a.hk;
+    id /= (uint32_t)a.hk;
+    const int slot0 = (int)(id % per_seq) * kSlots;
+    const int64_t b = id / per_seq;
     if (b >= a.batch) return;
-    const int t = a.kept[(b * a.hk + hkv) * a.budget + slot];
-    if (t < 0) return;
-    const int64_t src = (int64_t)a.block_table[b * a.block_table_stride + t / a.page_size] * a.page_size + t % a.page_size;
-    const int64_t dst = (int64_t)a.new_block_table[b * a.new_block_table_stride + slot / a.new_page_size] * a.new_page_size + slot % a.new_page_size;
-    if (piece < kp)
-        ((Piece*)a.new_k)[(dst * a.hk + hkv) * kp + piece] = ((const Piece*)a.k)[(src * a.hk + hkv) * kp + piece];
-    else
-        ((Piece*)a.new_v)[(dst * a.hk + hkv) * vp + piece - kp] = ((const Piece*)a.v)[(src * a.hk + hkv) * vp + piece - kp];
+    const int32_t* const kept = a.kept + (b * a.hk + hkv) * a.budget;
+    int t[kSlots];
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) t[s] = slot0 + s < a.budget ? kept[slot0 + s] : -1;
+    auto locate = [](const int32_t* table, int pos, int page, int shift) -> int64_t {
+        const int pi = shift >= 0 ? pos >> shift : pos / page;
+        return (int64_t)table[pi] * page + (pos - pi * page);
+    };
+    int64_t src[kSlots], dst[kSlots];
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+        src[s] = dst[s] = 0;
+        if (t[s] >= 0) {
+            src[s] = locate(a.block_table + b * a.block_table_stride, t[s], a.page_size, a.page_shift) * a.hk + hkv;
+            dst[s] = locate(a.new_block_table + b * a.new_block_table_stride, slot0 + s, a.new_page_size, a.new_page_shift) * a.hk + hkv;
+        }
+    }
+    Piece k[kSlots], v[kSlots];
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+        if (t[s] >= 0 && piece < kp) k[s] = __builtin_nontemporal_load((const Piece*)a.k + src[s] * kp + piece);
+        if (t[s] >= 0 && piece < vp) v[s] = __builtin_nontemporal_load((const Piece*)a.v + src[s] * vp + piece);
+    }
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+        if (t[s] >= 0 && piece < kp) ((Piece*)a.new_k)[dst[s] * kp + piece] = k[s];
+        if (t[s] >= 0 && piece < vp) ((Piece*)a.new_v)[dst[s] * vp + piece] = v[s];
+    }
 }
 
 template <typename Piece>
 hipError_t launch_move(const CacheEvictArgs& a, hipStream_t st)
 {
-    const int64_t items = (int64_t)a.batch * a.budget * a.hk * ((a.k_row + a.v_row) / (int)sizeof(Piece));
-    const int64_t grid = (items + 255) / 256;
-    if (grid > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((evict_move_kernel<Piece>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    const int64_t pieces = (a.k_row > a.v_row ? a.k_row : a.v_row) / (int)sizeof(Piece);
+    const int64_t items = (int64_t)a.batch * ((a.budget + kSlots - 1) / kSlots) * a.hk * pieces;
+    if (items > INT32_MAX) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((evict_move_kernel<Piece>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 

@@ -1018,11 +1018,21 @@ int fck_fmha_decode_shared_prefix(const void* q, const void* k_cache, const void
                                                    static_cast<hipStream_t>(stream)), "shared-prefix decode launch");
 }
 
-int fck_fmha_key_weights(const void* q, const void* k, const void* lse, const void* weights, void* out, const int32_t* seqstart_q,
+int fck_fmha_key_weights_row_splits(int64_t batch, int64_t hq, int64_t hk, int64_t sq, int64_t cols, int64_t d, uint32_t mask_type, int64_t num_cu)
+{
+    constexpr int64_t kMax = (int64_t)1 << 24;
+    for (int64_t v : {batch, hq, hk, d})
+        if (v <= 0 || v > kMax) return 1;
+    if (hk > hq || d > 256 || sq <= 0 || sq > INT32_MAX || cols <= 0 || cols > INT32_MAX || num_cu > kMax) return 1;
+    if (batch * hk > INT32_MAX) return 1;
+    return fck::key_weights_row_splits(kernel_dim(d, d), batch, hk, hq / hk, sq, cols, mask_type != 0, num_cu > 0 ? (int)num_cu : cu_count());
+}
+
+int fck_fmha_key_weights(const void* q, const void* k, const void* lse, const void* weights, void* out, void* workspace, const int32_t* seqstart_q,
                          const int32_t* seqlen_k_ptr, const int32_t* block_table, int64_t batch_stride_block_table,
                          int64_t page_block_size, int64_t batch, int64_t seqlen_q, int64_t seqlen_k, int64_t cols, int64_t hq, int64_t hk,
-                         int64_t d, int64_t q_max_seq_len, float scale, int64_t window_left, int64_t window_right, uint32_t mask_type,
-                         int32_t dtype, const fck_fmha_attrs* attrs, void* stream)
+                         int64_t d, int64_t q_max_seq_len, int64_t num_row_splits, float scale, int64_t window_left, int64_t window_right,
+                         uint32_t mask_type, int32_t dtype, const fck_fmha_attrs* attrs, void* stream)
 {
     g_err[0] = 0;
     if (dtype == FCK_DTYPE_FP8) return fail(FCK_ERR_UNSUPPORTED, "key weights take fp16 or bf16 queries (an e4m3 cache goes through fck_fmha_attrs.kv_dtype)");
@@ -1036,7 +1046,11 @@ int fck_fmha_key_weights(const void* q, const void* k, const void* lse, const vo
     if (q_max_seq_len <= 0) q_max_seq_len = seqlen_q;
     if (int rc = check_fit32(seqlen_q, seqlen_k, q_max_seq_len, cols, batch_stride_block_table, page_block_size, (seqstart_q ? 1 : batch) * seqlen_q,
                              q_max_seq_len * (hq / hk))) return rc;
+    if (num_row_splits < 1 || num_row_splits > 16) return fail(FCK_ERR_INVALID_ARGUMENT, "num_row_splits %ld out of range [1,16]", (long)num_row_splits);
+    if (num_row_splits > 1 && !workspace) return fail(FCK_ERR_INVALID_ARGUMENT, "num_row_splits > 1 needs a workspace");
     fck::KeyWeightsArgs a{};
+    a.partial = static_cast<float*>(workspace);
+    a.row_splits = (int32_t)num_row_splits;
     a.q = q;
     a.k = k;
     a.lse = static_cast<const float*>(lse);
@@ -1122,6 +1136,8 @@ int fck_fmha_cache_evict(const void* k_cache, const void* v_cache, void* new_k_c
     a.new_block_table_stride = (int32_t)new_batch_stride_block_table;
     a.page_size = (int32_t)page_block_size;
     a.new_page_size = (int32_t)new_page_block_size;
+    a.page_shift = log2_exact(page_block_size);
+    a.new_page_shift = log2_exact(new_page_block_size);
     a.batch = (int32_t)batch;
     a.hk = (int32_t)hk;
     a.budget = (int32_t)budget;

@@ -57,6 +57,16 @@ __device__ __forceinline__ void load_to_lds(uint32_t dst, const void* src)
                  : "memory");
 }
 
+// the same for data that is read once (the non-temporal hint: see ldg16_stream in common.hpp)
+__device__ __forceinline__ void load_to_lds_stream(uint32_t dst, const void* src)
+{
+    uint32_t m0_saved;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off nt\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0_saved)
+                 : "s"(dst), "v"(src)
+                 : "memory");
+}
+
 // A lane that sits out a global -> LDS instruction which other lanes of its wave issue (it is masked off for that
 // instruction): nothing to do on the hardware, where the wave's counter of outstanding operations counts the instruction
 // once for all lanes; the emulated twin keeps the lane's own count in step with it.
@@ -67,6 +77,14 @@ template <int N>
 __device__ __forceinline__ void wait_vm()
 {
     __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
+// wait until this wave's LDS (and scalar-memory) operations are complete: before a global -> LDS copy may overwrite what
+// they read
+__device__ __forceinline__ void wait_lds()
+{
+    __builtin_amdgcn_s_waitcnt(15 | (3 << 14) | (7 << 4));
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // acc *= f for a value that lives in the accumulation half of the register file, without moving it out for longer

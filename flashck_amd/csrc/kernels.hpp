@@ -7,11 +7,11 @@
 
 namespace fck {
 
-// Launch `Kern` with `lds` bytes of dynamic LDS.  More than 64 KiB needs an opt-in per kernel and device; it is made
+// Launch `Kern` with `lds` bytes of dynamic LDS (at most `max_lds` in any call, where that varies).  More than 64 KiB needs an opt-in per kernel and device; it is made
 // once per device under std::call_once, so concurrent first calls from several host threads are safe, and every later
 // call is a plain launch (nothing but the launch itself reaches the stream, so a warmed-up call can be captured).
 template <auto Kern, typename Args>
-inline hipError_t launch_with_lds(dim3 grid, dim3 block, size_t lds, hipStream_t st, const Args& a)
+inline hipError_t launch_with_lds(dim3 grid, dim3 block, size_t lds, hipStream_t st, const Args& a, size_t max_lds = 0)
 {
     constexpr int kMaxDev = 64;
     static std::once_flag once[kMaxDev];
@@ -21,7 +21,7 @@ inline hipError_t launch_with_lds(dim3 grid, dim3 block, size_t lds, hipStream_t
     if (e != hipSuccess) return e;
     if (dev < 0 || dev >= kMaxDev) return hipErrorInvalidDevice;
     std::call_once(once[dev], [&] {
-        status[dev] = hipFuncSetAttribute((const void*)Kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        status[dev] = hipFuncSetAttribute((const void*)Kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(max_lds > lds ? max_lds : lds));
     });
     if (status[dev] != hipSuccess) return status[dev];
     hipLaunchKernelGGL(Kern, grid, block, lds, st, a);
@@ -159,9 +159,13 @@ struct KeyWeightsArgs {
     int64_t window_left, window_right;
     ScoreMod mod;  // ALiBi / soft cap
     int32_t kv8;
-    int32_t rows_max;  // most packed query rows of a sequence
+    int32_t rows_max;    // most packed query rows of a sequence
+    int32_t row_splits;  // runs the query tokens are cut into (prompts)
+    float* partial;      // row_splits > 1: [row_splits, B, Hk, cols]
     int32_t num_cu;
 };
+// runs the query tokens of a call are worth cutting into (1: none)
+int key_weights_row_splits(int d, int64_t batch, int64_t hk, int64_t g, int64_t sq, int64_t cols, bool masked, int num_cu);
 hipError_t launch_key_weights(const KeyWeightsArgs& a, int d, int dtype, hipStream_t st);
 
 // Choice of the keys a cache keeps, and their move to new pages (cache_evict.hip).
@@ -178,6 +182,7 @@ struct CacheEvictArgs {
     const int32_t* block_table;
     const int32_t* new_block_table;
     int32_t block_table_stride, new_block_table_stride, page_size, new_page_size;
+    int32_t page_shift, new_page_shift;  // log2 of the page sizes, -1 when they are no powers of two
     int32_t batch, hk, budget, recent, sinks;
     int64_t cols;
     int32_t k_row, v_row;  // bytes of one head's row of K and V (multiples of 8)

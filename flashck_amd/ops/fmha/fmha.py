@@ -1001,7 +1001,7 @@ def fmha_decode_shared_prefix(q, k_cache, v_cache, seqlen_k, block_table, prefix
 
 def fmha_key_weights(q, k_cache, lse, seqlen_k, block_table=None, *, weights=None, cu_seqlens_q=None, max_seqlen_q: int = 0,
                      max_seqlen_k: int = 0, scale: float = 0.0, mask_type: int = MASK_NONE, window=(-1, -1), alibi_slopes=None,
-                     logits_soft_cap: float = 0.0, k_descale: float = 1.0, out=None) -> torch.Tensor:
+                     logits_soft_cap: float = 0.0, k_descale: float = 1.0, num_row_splits: int = 0, out=None) -> torch.Tensor:
     """Attention weight every cached key receives, fp32 [B, Hk, cols]:
 
         out[b, hk, t] = weights[b, hk, t] + sum over the query heads h of KV head hk and the rows i that see t of
@@ -1012,7 +1012,8 @@ def fmha_key_weights(q, k_cache, lse, seqlen_k, block_table=None, *, weights=Non
     k_cache is a paged cache with block_table, or [B, sk, Hk, D] without one (seqlen_k may then be None).
     weights (optional) are what earlier steps accumulated; out may be the same tensor.  cols is their last dimension, else
     max_seqlen_k, else what the cache can hold.  Entries at and behind a sequence's key count are written as 0, so the tensor
-    can go on growing with its cache.  Masks, windows, ALiBi, soft cap and quantised keys as the attention operators."""
+    can go on growing with its cache.  Masks, windows, ALiBi, soft cap and quantised keys as the attention operators.
+    num_row_splits: runs a long stretch of queries is cut into (0: chosen from the CU count)."""
     if seqlen_k is None and block_table is not None:
         raise ValueError("a paged cache needs seqlen_k")
     _check_tensor("seqlen_k", seqlen_k, dtype=torch.int32, ndim=1, optional=True)
@@ -1050,11 +1051,14 @@ def fmha_key_weights(q, k_cache, lse, seqlen_k, block_table=None, *, weights=Non
     if block_table is not None:
         _debug_validate(seqlen_k=seqlen_k, block_table=block_table, num_total_pages=k_cache.shape[0], page_size=page)
     o = _out("out", out, (B, Hk, cols), torch.float32, q)
+    if num_row_splits <= 0:
+        num_row_splits = int(_lib.load().fck_fmha_key_weights_row_splits(B, Hq, Hk, sq_max, cols, D, mask_type, 0))
+    partial = torch.empty(num_row_splits, B, Hk, cols, dtype=torch.float32, device=q.device) if num_row_splits > 1 else None
     wl, wr = _window(window)
     at, keep = _attrs(q, None, alibi_slopes, logits_soft_cap, group, B, sq, 1, kv_fp8, k_descale, 1.0)
     with _on(q):
-        _call("fck_fmha_key_weights", _ptr(q), _ptr(k_cache), _ptr(lse), _ptr(weights), _ptr(o), _ptr(cu_seqlens_q), _ptr(seqlen_k),
-              _ptr(block_table), stride, page, B, sq, sk, cols, Hq, Hk, D, sq_max, _scale(scale, D), wl, wr, mask_type, _dtype_id(q),
+        _call("fck_fmha_key_weights", _ptr(q), _ptr(k_cache), _ptr(lse), _ptr(weights), _ptr(o), _ptr(partial), _ptr(cu_seqlens_q), _ptr(seqlen_k),
+              _ptr(block_table), stride, page, B, sq, sk, cols, Hq, Hk, D, sq_max, num_row_splits, _scale(scale, D), wl, wr, mask_type, _dtype_id(q),
               at, _stream())
     del keep
     return o

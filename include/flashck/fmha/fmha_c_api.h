@@ -323,17 +323,22 @@ FCK_EXPORT int fck_fmha_shared_prefix_splits(int64_t batch, int64_t num_groups, 
  *            (fck_fmha_attrs.lse, _combine_lse, fck_fmha_decode_shared_prefix); a row with -inf adds nothing
  *   weights, out  fp32 [B, Hk, cols]; weights may be NULL (zeros) or out itself.  Entries at and behind a sequence's key
  *            count are written as 0; keys at and behind cols have no entry.
+ *   workspace  fp32 [num_row_splits, B, Hk, cols] when num_row_splits > 1 (in [1, 16]; fck_fmha_key_weights_row_splits chooses:
+ *            long runs of queries are cut so that few keys fill the chip), else NULL
  *   k        paged cache with block_table + seqlen_k_ptr, or (block_table NULL) batch cache [B, seqlen_k, Hk, D] with optional
  *            seqlen_k_ptr.  seqlen_q carries total_q in group mode.
  * attrs: ALiBi, soft cap, kv_dtype with k_descale.  No counterpart in the reference.
  */
 FCK_EXPORT int fck_fmha_key_weights(const void* q, const void* k, const void* lse, const void* weights, void* out,
-                                    const int32_t* seqstart_q, const int32_t* seqlen_k_ptr, const int32_t* block_table,
+                                    void* workspace, const int32_t* seqstart_q, const int32_t* seqlen_k_ptr, const int32_t* block_table,
                                     int64_t batch_stride_block_table, int64_t page_block_size, int64_t batch,
                                     int64_t seqlen_q, int64_t seqlen_k, int64_t cols, int64_t q_num_heads,
-                                    int64_t kv_num_heads, int64_t qk_head_dim, int64_t q_max_seq_len, float scale,
-                                    int64_t window_left, int64_t window_right, uint32_t mask_type, int32_t dtype,
-                                    const fck_fmha_attrs* attrs, void* stream);
+                                    int64_t kv_num_heads, int64_t qk_head_dim, int64_t q_max_seq_len,
+                                    int64_t num_row_splits, float scale, int64_t window_left, int64_t window_right,
+                                    uint32_t mask_type, int32_t dtype, const fck_fmha_attrs* attrs, void* stream);
+FCK_EXPORT int fck_fmha_key_weights_row_splits(int64_t batch, int64_t q_num_heads, int64_t kv_num_heads,
+                                               int64_t q_max_seq_len, int64_t cols, int64_t qk_head_dim,
+                                               uint32_t mask_type, int64_t num_cu);
 
 /*
  * Eviction: every (sequence, KV head) keeps n = min(seqlen_k[b], budget) keys: all of them when seqlen_k[b] <= budget, else

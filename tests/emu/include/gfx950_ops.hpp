@@ -40,6 +40,8 @@ inline void load_to_lds(uint32_t dst, const void* base, uint32_t off)
 }
 inline void load_to_lds(uint32_t dst, const void* src) { emu::request_copy((char*)(uintptr_t)dst + emu::cur->lane * 16, (const char*)src); }
 
+inline void load_to_lds_stream(uint32_t dst, const void* src) { load_to_lds(dst, src); }
+
 // a masked-off lane of an issued instruction: an empty entry in the lane's queue
 #define FCK_LOAD_TO_LDS_MASKED() emu::request_copy(nullptr, nullptr)
 
@@ -49,6 +51,9 @@ inline void wait_vm()
 {
     emu::land_copies(N);
 }
+
+// all lanes of the wave have made their LDS reads before any of them goes on
+inline void wait_lds() { (void)emu::exchange("", 1); }
 
 #define FCK_ACC_SCALE(acc, f) ((acc) *= (f))
 #define FCK_PIN_VGPR(x) ((void)0)

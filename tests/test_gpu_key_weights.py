@@ -142,3 +142,41 @@ def test_results_are_the_same_every_time(fmha):
     _check(first, lc.key_weights(c["q"], c["keys"], c["lse"], first.shape[2], 128 ** -0.5, **kw), lens)
     for _ in range(3):
         assert torch.equal(first, fmha.fmha_key_weights(*args, **kw).cpu())
+
+
+@pytest.mark.parametrize("mask_type,window", [(0, (-1, -1)), (2, (-1, 0)), (2, (60, 5)), (1, (-1, 0))])
+@pytest.mark.parametrize("sq,hq,hk,d,page", [(290, 2, 1, 64, 64), (290, 3, 3, 128, 16), (100, 3, 1, 128, 128), (70, 1, 1, 256, 48),
+                                             (290, 2, 1, 72, 64)])
+def test_long_query_runs(fmha, mask_type, window, sq, hq, hk, d, page):
+    # more rows than LDS holds: stages that are full and not, runs that end inside a stage, keys that some waves do not have
+    lens = [sq, 277]
+    kw = dict(mask_type=mask_type, window=window)
+    c = _case(11, lens, sq, hq, hk, d, torch.bfloat16, page, **kw)
+    cols = max(lens) + 3
+    want = lc.key_weights(c["q"], c["keys"], c["lse"], cols, d ** -0.5, **kw)
+    before = torch.rand(2, hk, cols, generator=torch.Generator().manual_seed(1))
+    for splits in (1, 3):
+        out = fmha.fmha_key_weights(dev(c["q"]), dev(c["kc"]), dev(c["lse"]), _i32(lens), dev(c["table"]), max_seqlen_k=cols,
+                                    num_row_splits=splits, **kw)
+        _check(out, want, lens, f"{kw} splits {splits}")
+        w = dev(before)
+        fmha.fmha_key_weights(dev(c["q"]), dev(c["kc"]), dev(c["lse"]), _i32(lens), dev(c["table"]), weights=w, out=w,
+                              num_row_splits=splits, **kw)
+        want_w = want.clone()
+        for b, n in enumerate(lens):
+            want_w[b, :, :n] += before[b, :, :n].double()
+        _check(w, want_w, lens, f"{kw} splits {splits} in place")
+
+
+def test_long_packed_quantised_and_modified_runs(fmha):
+    starts, lens, slopes = [0, 270, 271], [300, 40], torch.tensor([0.25, 0.0625])
+    kw = dict(mask_type=2, window=(-1, 0))
+    c = _case(12, lens, 0, 2, 1, 64, torch.float16, 16, fp8=True, kd=0.5, starts=starts, **kw)
+    out = fmha.fmha_key_weights(dev(c["q"]), dev(c["kc"]), dev(c["lse"]), _i32(lens), dev(c["table"]), cu_seqlens_q=_i32(starts),
+                                max_seqlen_q=270, max_seqlen_k=300, k_descale=0.5, num_row_splits=2, **kw)
+    _check(out, lc.key_weights(c["q"], c["keys"], c["lse"], 300, 0.125, starts=starts, **kw), lens)
+    c = _case(13, lens, 0, 2, 1, 64, torch.bfloat16, 64, starts=starts, cap=3.0, slopes=slopes, **kw)
+    out = fmha.fmha_key_weights(dev(c["q"]), dev(c["kc"]), dev(c["lse"]), _i32(lens), dev(c["table"]), cu_seqlens_q=_i32(starts),
+                                max_seqlen_q=270, max_seqlen_k=300, alibi_slopes=dev(slopes), logits_soft_cap=3.0, **kw).cpu()
+    want = lc.key_weights(c["q"], c["keys"], c["lse"], 300, 0.125, starts=starts, cap=3.0, slopes=slopes, **kw)
+    assert ((out.double() - want).abs() - 2e-4 * want).max() <= 1e-9  # the slopes add up to 75: fp32 steps of 2^-17 there
