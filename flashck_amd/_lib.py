@@ -40,8 +40,8 @@ SIGNATURES = {
     "fck_fmha_validate_paged": (ctypes.c_int, [_vp] * 6 + [_i64] * 3 + [_vp, _vp]),
     "fck_fmha_fwd_splitkv_combine": (ctypes.c_int, [_vp] * 4 + [_i64] * 6 + [_i32, _vp]),
     "fck_fmha_fwd_splitkv_combine_lse": (ctypes.c_int, [_vp] * 5 + [_i64] * 6 + [_i32, _vp]),
-    "fck_fmha_decode_shared_prefix": (ctypes.c_int, [_vp] * 12 + [_i64] * 13 + [_f32, _i64, _i64, _u32, _i32, _ap, _vp]),
-    "fck_fmha_shared_prefix_splits": (ctypes.c_int, [_i64] * 9 + [_vp] * 2),
+    "fck_fmha_decode_shared_prefix": (ctypes.c_int, [_vp] * 12 + [_i64] * 15 + [_f32, _i64, _i64, _u32, _i32, _ap, _vp]),
+    "fck_fmha_shared_prefix_splits": (ctypes.c_int, [_i64] * 10 + [_vp] * 2),
     "fck_fmha_key_weights_row_splits": (ctypes.c_int, [_i64] * 6 + [_u32, _i64]),
     "fck_fmha_key_weights": (ctypes.c_int, [_vp] * 9 + [_i64] * 11 + [_f32, _i64, _i64, _u32, _i32, _ap, _vp]),
     "fck_fmha_cache_evict": (ctypes.c_int, [_vp] * 10 + [_i64] * 2 + [_vp] + [_i64] * 10 + [_i32, _vp]),

@@ -8,6 +8,8 @@
 #include "common.hpp"
 #include "kernels.hpp"
 
+#include <type_traits>
+
 namespace fck {
 namespace {
 
@@ -17,23 +19,25 @@ constexpr int kWaves = kThreads / 64;
 // order-preserving map of a weight to an unsigned key; -0 and +0 are equal, NaN is -inf
 __device__ __forceinline__ uint32_t weight_key(float w)
 {
-    if (w != w) w = -INFINITY;
-    if (w == 0.f) w = 0.f;
-    const uint32_t u = __builtin_bit_cast(uint32_t, w);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
+    const float x = fmaxf(w + 0.f, -INFINITY);  // the sum turns -0 into +0, the maximum a NaN into -inf
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
+
+// The histogram of one digit: kBins counters in kColumns copies, a lane adds to copy lane % kColumns.
+constexpr int kBits = 11, kBins = 1 << kBits, kColumns = 8;
 
 // One workgroup per (sequence, KV head); bound by the walks over its weights (L2 round trips), so they are few and wide: a wave
 // owns a contiguous sixteenth of the row and reads 4 weights per lane and load.
-//   1. The want-th largest key of the middle, 8 bits per walk, from a histogram in LDS with a column per lane: lanes never
-//      meet at an address or a bank whatever the weights are (a single histogram serialised on the many equal weights, zeros
-//      above all: 369 us for one sequence of 131072 keys and 8 heads).
+//   1. The want-th largest key of the middle, 11 bits per walk, from a histogram in LDS with a copy for every 8th lane, so
+//      that equal weights, zeros above all, meet at an address seldom (one copy and 8 bits per walk: 369 us for a sequence of
+//      131072 keys and 8 heads; a copy per lane: 154 us).
 //   2. A walk that counts what each wave keeps, and one that writes it from the wave's first rank on: ranks are ballots, and
 //      no barrier lies inside a walk.
 __global__ __launch_bounds__(kThreads) void evict_select_kernel(const CacheEvictArgs a)
 {
-    __shared__ int hist[256 * 64];  // [digit][lane]
-    __shared__ __align__(16) int digits[256];
+    __shared__ int hist[kBins * kColumns];  // [digit][copy]
+    __shared__ __align__(16) int digits[kBins], groups[kBins / 64];
     __shared__ int chosen[3];
     __shared__ int counts[2][kWaves];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -62,18 +66,24 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(const CacheEvict
         for (int e = 0; e < 4; ++e) x[e] = t + e < a.cols ? w[t + e] : 0.f;
         return x;
     };
-    // calls f(position of the lane's first weight, its 4 weights) for the wave's segment; positions from len on are the
-    // caller's to leave out.  Four loads are in flight per lane.
+    // calls f(position of the lane's first weight, its 4 weights, whether all of the wave's 256 lie in the middle) for the
+    // wave's segment; other positions may lie behind the row, which is f's to leave out.  Four loads are in flight per lane.
     auto walk = [&](auto f) {
+        auto call = [&](int t0, const f32x4_t& x) {
+            if (t0 >= lo && t0 + 256 <= hi)
+                f(t0 + lane * 4, x, std::true_type{});
+            else
+                f(t0 + lane * 4, x, std::false_type{});
+        };
         int t0 = seg0;
         for (; t0 + 1024 <= seg1; t0 += 1024) {
             f32x4_t x[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) x[u] = load4(t0 + u * 256 + lane * 4);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) f(t0 + u * 256 + lane * 4, x[u]);
+            for (int u = 0; u < 4; ++u) call(t0 + u * 256, x[u]);
         }
-        for (; t0 < seg1; t0 += 256) f(t0 + lane * 4, load4(t0 + lane * 4));
+        for (; t0 < seg1; t0 += 256) call(t0, load4(t0 + lane * 4));
     };
 
     uint32_t threshold = 0;  // the want-th largest key, in the digits that decide
@@ -81,52 +91,74 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(const CacheEvict
     if (want > 0) {
         uint32_t mask = 0;
         int left = want;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int e = tid; e < 256 * 64; e += kThreads) hist[e] = 0;
+        for (int shift = 32 - kBits; mask != 0xffffffffu; shift = max(shift - kBits, 0)) {
+            const uint32_t digit_mask = (kBins - 1u) << shift & ~mask;
+            for (int e = tid; e < kBins * kColumns; e += kThreads) hist[e] = 0;
             __syncthreads();
-            walk([&](int t, const f32x4_t& x) {
+            walk([&](int t, const f32x4_t& x, auto middle) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint32_t key = weight_key(x[e]);
-                    if (t + e >= lo && t + e < hi && (key & mask) == threshold) atomicAdd(&hist[(key >> shift & 255) * 64 + lane], 1);
+                    const bool in = decltype(middle)::value || (t + e >= lo && t + e < hi);
+                    if (in && (key & mask) == threshold) atomicAdd(&hist[((key & digit_mask) >> shift) * kColumns + lane % kColumns], 1);
                 }
             });
             __syncthreads();
-            if (tid < 256) {
+            // the digit of the left-th largest: by groups of 64 digits first
+            for (int d = tid; d < kBins; d += kThreads) {
                 int sum = 0;
-                for (int c = 0; c < 64; ++c) sum += hist[tid * 64 + ((c + tid) & 63)];
-                digits[tid] = sum;
+#pragma unroll
+                for (int c = 0; c < kColumns; ++c) sum += hist[d * kColumns + ((c + d) & (kColumns - 1))];
+                digits[d] = sum;
             }
             __syncthreads();
-            if (tid < 256) {
+            if (tid < kBins / 64) {
+                int sum = 0;
+                for (int d = 0; d < 64; ++d) sum += digits[tid * 64 + ((d + tid) & 63)];
+                groups[tid] = sum;
+            }
+            __syncthreads();
+            if (tid < kBins / 64) {
                 int above = 0;
-                for (int d = 0; d < 256; d += 4) {
-                    const u32x4_t n = *reinterpret_cast<const u32x4_t*>(&digits[d]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) above += d + e > tid ? (int)n[e] : 0;
-                }
-                const int here = digits[tid];
-                if (above < left && left <= above + here) {  // exactly one thread
-                    chosen[0] = tid;
+                for (int j = 0; j < kBins / 64; ++j) above += j > tid ? groups[j] : 0;
+                if (above < left && left <= above + groups[tid]) {  // exactly one thread
+                    chosen[0] = tid * 64;
                     chosen[1] = left - above;
+                }
+            }
+            __syncthreads();
+            const int first = chosen[0], in_group = chosen[1];
+            __syncthreads();
+            if (tid < 64) {
+                int above = 0;
+                for (int j = 0; j < 64; j += 4) {
+                    const u32x4_t n = *reinterpret_cast<const u32x4_t*>(&digits[first + j]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) above += j + e > tid ? (int)n[e] : 0;
+                }
+                const int here = digits[first + tid];
+                if (above < in_group && in_group <= above + here) {  // exactly one thread
+                    chosen[0] = first + tid;
+                    chosen[1] = in_group - above;
                     chosen[2] = here;
                 }
             }
             __syncthreads();
             threshold |= (uint32_t)chosen[0] << shift;
             left = chosen[1];
-            mask |= 255u << shift;
+            mask |= digit_mask;
             if (chosen[2] == left) break;  // every key that begins like this is kept: the digits behind do not matter
+            __syncthreads();
         }
         equal_wanted = left;
         const uint32_t m = mask;
         int sure = 0, equal = 0;
-        walk([&](int t, const f32x4_t& x) {
+        walk([&](int t, const f32x4_t& x, auto in) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int p = t + e;
                 const uint32_t key = weight_key(x[e]) & m;
-                const bool middle = p >= lo && p < hi;
+                const bool middle = decltype(in)::value || (p >= lo && p < hi);
                 sure += __builtin_popcountll(__builtin_amdgcn_ballot_w64(p < len && (!middle || key > threshold)));
                 equal += __builtin_popcountll(__builtin_amdgcn_ballot_w64(middle && key == threshold));
             }
@@ -142,7 +174,7 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(const CacheEvict
             rank += counts[0][v] + eq;
             equal_left -= eq;
         }
-        walk([&](int t, const f32x4_t& x) {
+        walk([&](int t, const f32x4_t& x, auto in) {
             // per element: kept without question, or equal to the threshold and early enough
             uint64_t keep_mask[4], eq_mask[4];
             bool mine[4], eq[4];
@@ -150,7 +182,7 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(const CacheEvict
             for (int e = 0; e < 4; ++e) {
                 const int p = t + e;
                 const uint32_t key = weight_key(x[e]) & m;
-                const bool middle = p >= lo && p < hi;
+                const bool middle = decltype(in)::value || (p >= lo && p < hi);
                 mine[e] = p < len && (!middle || key > threshold);
                 eq[e] = middle && key == threshold;
                 eq_mask[e] = __builtin_amdgcn_ballot_w64(eq[e]);

@@ -179,9 +179,11 @@ __device__ __forceinline__ float fast_log2(float x) { return __builtin_amdgcn_lo
 // the split-KV kernel, so both produce the same bits.
 constexpr int kCombineBatch = 16;
 
+// lse (null: not asked for) receives the merged LSE, -inf when every split is empty.
 template <int DV>
 __device__ __forceinline__ f32x4_t combine_splits(const float* lse_acc, const float* o_acc, int64_t w0, int64_t step, int ns, int c,
-                                                  int dv = DV)  // dv: floats per partial row as stored (<= DV)
+                                                  int dv = DV,  // dv: floats per partial row as stored (<= DV)
+                                                  float* lse = nullptr)
 {
     float m_run = -INFINITY, sum = 0.f;
     f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
@@ -216,20 +218,11 @@ __device__ __forceinline__ f32x4_t combine_splits(const float* lse_acc, const fl
         }
         m_run = m_new;
     }
+    if (lse) *lse = sum == 0.f ? -INFINITY : m_run + fast_log2(sum) * kLn2;
     if (sum == 0.f) return f32x4_t{0.f, 0.f, 0.f, 0.f};
     if (ns == 1) return acc;  // weight exactly 1
     const float inv = 1.f / sum;
     return f32x4_t{acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
-}
-
-// Log-sum-exp over a row's splits, as combine_splits weighs them; -inf when all of them are empty (or there is none).
-__device__ __forceinline__ float combine_lse(const float* lse_acc, int64_t w0, int64_t step, int ns)
-{
-    float m = -INFINITY, sum = 0.f;
-    for (int s = 0; s < ns; ++s) m = fmaxf(m, lse_acc[w0 + s * step]);
-    if (m == -INFINITY) return -INFINITY;
-    for (int s = 0; s < ns; ++s) sum += __expf(lse_acc[w0 + s * step] - m);
-    return m + fast_log2(sum) * kLn2;
 }
 
 // Visible key range [lo, hi) of query row i: GenericAttentionMask::IsOutOfBound,

@@ -929,24 +929,27 @@ int fck_fmha_fwd_pagedkv_attrs(const void* q, const void* k_cache, const void* v
 }
 
 int fck_fmha_shared_prefix_splits(int64_t batch, int64_t num_groups, int64_t max_group_size, int64_t hq, int64_t hk, int64_t sq,
-                                  int64_t max_prefix_len, int64_t max_own_len, int64_t num_cu, int32_t* prefix_splits, int32_t* own_splits)
+                                  int64_t head_dim, int64_t max_prefix_len, int64_t max_own_len, int64_t num_cu,
+                                  int32_t* prefix_splits, int32_t* own_splits)
 {
     if (prefix_splits) *prefix_splits = 1;
     if (own_splits) *own_splits = 1;
     constexpr int64_t kMax = (int64_t)1 << 24;
     for (int64_t v : {batch, num_groups, max_group_size, hq, hk, sq})
         if (v <= 0 || v > kMax) return FCK_OK;
-    if (hk > hq || max_prefix_len > INT32_MAX || max_own_len > INT32_MAX || num_cu > kMax) return FCK_OK;
-    if (num_cu <= 0) num_cu = cu_count();
-    const auto choose = [&](int64_t streams, int64_t rows, int64_t keys) {
-        const int64_t items = streams * hk * ((rows + 63) / 64);
-        const int64_t want = (2 * num_cu + items - 1) / items, cap = keys / 256;
-        const int64_t ns = want < cap ? want : cap;
-        return (int32_t)(ns < 1 ? 1 : ns > 64 ? 64 : ns);
-    };
-    const int64_t g = hq / hk;
-    if (prefix_splits) *prefix_splits = choose(num_groups, max_group_size * sq * g, max_prefix_len);
-    if (own_splits) *own_splits = choose(batch, sq * g, max_own_len);
+    if (hk > hq || head_dim <= 0 || head_dim > 256 || max_prefix_len > INT32_MAX || max_own_len > INT32_MAX || num_cu > kMax) return FCK_OK;
+    // The items (a split x a KV head x a row tile) of the longest prefixes and of half the longest own keys should fill the
+    // workgroups that run at once, one round of equal ones.
+    const int64_t rows = max_group_size * sq * (hq / hk);
+    const int d = kernel_dim(head_dim, head_dim), bm = 64 * fck::shared_prefix_blocks(d, rows);
+    const double slots = fck::shared_prefix_workgroups(d, rows, num_cu > 0 ? (int)num_cu : cu_count());
+    const auto tiles = [&](int64_t r) { return (double)((r + bm - 1) / bm); };
+    const double prefix = max_prefix_len > 0 ? (double)max_prefix_len : 0, own = max_own_len > 0 ? (double)max_own_len : 0;
+    const double keys = (double)hk * (num_groups * tiles(rows) * prefix + batch * tiles(sq * (hq / hk)) * own / 2);
+    const double chunk = std::fmax(64.0, std::ceil(keys / slots / 64) * 64);
+    const auto splits = [&](double n) { return (int32_t)std::fmin(64.0, std::fmax(1.0, std::ceil(n / chunk))); };
+    if (prefix_splits) *prefix_splits = splits(prefix);
+    if (own_splits) *own_splits = splits(own);
     return FCK_OK;
 }
 
@@ -954,8 +957,8 @@ int fck_fmha_decode_shared_prefix(const void* q, const void* k_cache, const void
                                   const int32_t* seqstart_q, const int32_t* seqlen_k_ptr, const int32_t* block_table,
                                   const int32_t* cu_groups, const int32_t* prefix_lens, int64_t batch, int64_t num_groups,
                                   int64_t max_group_size, int64_t seqlen_q, int64_t hq, int64_t hk, int64_t d, int64_t dv,
-                                  int64_t q_max_seq_len, int64_t num_prefix_splits, int64_t num_own_splits,
-                                  int64_t batch_stride_block_table, int64_t page_block_size, float scale, int64_t window_left,
+                                  int64_t q_max_seq_len, int64_t num_prefix_splits, int64_t num_own_splits, int64_t max_prefix_len,
+                                  int64_t max_own_len, int64_t batch_stride_block_table, int64_t page_block_size, float scale, int64_t window_left,
                                   int64_t window_right, uint32_t mask_type, int32_t dtype, const fck_fmha_attrs* attrs, void* stream)
 {
     g_err[0] = 0;
@@ -975,7 +978,16 @@ int fck_fmha_decode_shared_prefix(const void* q, const void* k_cache, const void
         return fail(FCK_ERR_INVALID_ARGUMENT, "num_prefix_splits %ld / num_own_splits %ld out of range [1,64]", (long)num_prefix_splits, (long)num_own_splits);
     if (page_block_size <= 0 || batch_stride_block_table <= 0) return fail(FCK_ERR_INVALID_ARGUMENT, "page_block_size and batch_stride_block_table must be positive");
     if (int rc = check_fit32(page_block_size, batch_stride_block_table, seqlen_q, q_max_seq_len, num_groups, (seqstart_q ? 1 : batch) * seqlen_q)) return rc;
+    // keys per split; what lies behind the bounds goes to the last split
+    const int64_t capacity = batch_stride_block_table * page_block_size;
+    const auto chunk = [&](int64_t bound, int64_t ns) {
+        if (bound <= 0 || bound > capacity) bound = capacity;
+        const int64_t c = ((bound + ns - 1) / ns + 63) / 64 * 64;
+        return (int32_t)(c > INT32_MAX / 64 * 64 ? INT32_MAX / 64 * 64 : c);
+    };
     fck::SharedPrefixArgs a{};
+    a.prefix_chunk = chunk(max_prefix_len, num_prefix_splits);
+    a.own_chunk = chunk(max_own_len, num_own_splits);
     a.q = q;
     a.k = k_cache;
     a.v = v_cache;

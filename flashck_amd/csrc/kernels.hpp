@@ -128,6 +128,7 @@ struct SharedPrefixArgs {
     int32_t batch, groups, max_group;  // max_group: sequences of a group the prefix rows cover (the others read all of their own keys)
     int32_t sq, hq, hk, d, dv;
     int32_t ns_prefix, ns_own;
+    int32_t prefix_chunk, own_chunk;  // keys per split (multiples of 64)
     int32_t prefix_tiles, own_tiles;  // row tiles per (group, KV head) / per (sequence, KV head); set by the launcher
     int32_t prefix_items;             // workgroups that handle prefixes; set by the launcher
     int64_t shape_sq;                 // Sq of the workspace: sq (batch mode) or total_q
@@ -139,6 +140,9 @@ struct SharedPrefixArgs {
     float v_descale;
     int32_t num_cu;
 };
+// 16-row blocks per wave for groups of rows_prefix packed rows, and the workgroups that run at once with them
+int shared_prefix_blocks(int d, int64_t rows_prefix);
+int shared_prefix_workgroups(int d, int64_t rows_prefix, int num_cu);
 // rows_prefix / rows_own: most packed query rows of a group / of a sequence
 hipError_t launch_shared_prefix(SharedPrefixArgs a, int d, int dtype, int64_t rows_prefix, int64_t rows_own, hipStream_t st);
 

@@ -14,6 +14,7 @@
 //   after it has set them up.
 //   Prefix items come first (they are the long ones); those that stream the same keys get ids congruent modulo 8, i.e. one
 //   XCD and one L2.
+//   Every slot of every row is written (an empty one as lse = -inf), so the merge reads no lengths and no groups.
 #include "common.hpp"
 #include "kernels.hpp"
 
@@ -63,10 +64,10 @@ __device__ __forceinline__ int own_begin(const SharedPrefixArgs& a, int b)
     return b >= s.first && b < s.first + s.count ? s.prefix : 0;
 }
 
-template <int D>
+template <int D, int MB>
 struct SharedShape {
     static constexpr int TK = D == 256 ? 32 : 64;  // keys per tile
-    static constexpr int BM = 64;                  // query rows per workgroup, 16 per wave
+    static constexpr int BM = 64 * MB;             // query rows per workgroup, 16 MB per wave
     static constexpr int NBK = TK / 16;            // 16-key blocks per tile
     static constexpr int KT = D / 32;              // MFMA k-steps of the QK product
     static constexpr int DB = D / 16;              // 16-column blocks of the output
@@ -76,24 +77,31 @@ struct SharedShape {
     static constexpr int LD = TK * CH / 256;  // chunks per thread and operand
 };
 
+// waves per SIMD (= workgroups per CU) the registers leave
+template <int D, int MB>
+constexpr int kSharedWaves = MB == 2 || D == 256 ? 2 : 3;
+
 template <int D>
 __device__ __forceinline__ int shared_v_swizzle(int key)
 {
     return ((key & 7) << 1) & (D / 8 - 1);
 }
 
-// The kernel for every head dim, page size and cache type: 4 waves of 16 rows, K/V tiles through registers into
-// double-buffered LDS that all waves read.
+// 4 waves of 16 MB rows.  A K/V tile goes through registers into one LDS buffer that all waves read; the next tile is in
+// flight in the registers meanwhile.  One buffer and not two: three small workgroups per CU hide the latencies of short items
+// better than two large ones.
+// MB = 2 (groups of more than 64 rows, head dim <= 128): every fragment read from LDS feeds two matrix instructions, which
+// is what bounds the product of a large group with its prefix.
 // kUniform: pages are a multiple of the key tile.  kMod: ALiBi / soft cap.  kPad: stored head dims smaller than D (missing
 // chunks are zeros).  kKv8: e4m3 caches, widened to T on their way into LDS; always with kMod.
-template <typename T, int D, bool kUniform, bool kMod, bool kPad, bool kKv8>
-__global__ __launch_bounds__(256) void shared_prefix_kernel(const SharedPrefixArgs a)
+template <typename T, int D, int MB, bool kUniform, bool kMod, bool kPad, bool kKv8>
+__global__ __launch_bounds__(256, (kSharedWaves<D, MB>)) void shared_prefix_kernel(const SharedPrefixArgs a)
 {
-    typedef SharedShape<D> S;
+    typedef SharedShape<D, MB> S;
     typedef typename T::vec8 vec8;
     FCK_DYNAMIC_LDS(smem);
-    char FCK_LDS* const lds = (char FCK_LDS*)smem;  // K0 | K1 | V0 | V1 | visible range
-    int FCK_LDS* const range = (int FCK_LDS*)(lds + 4 * S::TILEB);
+    char FCK_LDS* const lds = (char FCK_LDS*)smem;  // K | V | visible range
+    int FCK_LDS* const range = (int FCK_LDS*)(lds + 2 * S::TILEB);
 
     const int dq = kPad ? a.d : D, dvs = kPad ? a.dv : D;
     const int tid = threadIdx.x;
@@ -119,7 +127,7 @@ __global__ __launch_bounds__(256) void shared_prefix_kernel(const SharedPrefixAr
         leader = sg.first;
         key_lo = 0;
         key_hi = sg.prefix;
-        if (key_hi <= 0) return;
+        if (key_hi <= 0) return;  // the own items of its sequences write these slots
         tok0 = a.seqstart_q ? a.seqstart_q[sg.first] : sg.first * a.sq;
         tok1 = a.seqstart_q ? a.seqstart_q[sg.first + sg.count] : (sg.first + sg.count) * a.sq;
     } else {
@@ -133,73 +141,76 @@ __global__ __launch_bounds__(256) void shared_prefix_kernel(const SharedPrefixAr
         ns = a.ns_own;
         slot = a.ns_prefix + split;
         key_lo = own_begin(a, b);
-        key_hi = shared_len(a, b);
-        if (key_hi <= key_lo) return;
+        key_hi = max(shared_len(a, b), key_lo);
         tok0 = a.seqstart_q ? a.seqstart_q[b] : b * a.sq;
         tok1 = a.seqstart_q ? a.seqstart_q[b + 1] : tok0 + a.sq;
     }
     const int64_t R = (int64_t)(tok1 - tok0) * g;
     const int64_t r0 = (int64_t)mt * S::BM;
     if (r0 >= R) return;
-    // splits are equal runs of whole tiles
+    // A split is a chunk of whole tiles, the same for every group or sequence: items of one size pack better than equal parts of
+    // ragged lengths.  The last one takes whatever lies behind the caller's bound; a short sequence leaves its last ones empty.
     const int base = key_lo / S::TK * S::TK;
-    const int64_t per = ((int64_t)(key_hi - base) + (int64_t)ns * S::TK - 1) / ((int64_t)ns * S::TK) * S::TK;
+    const int64_t per = prefix ? a.prefix_chunk : a.own_chunk;
     const int k0 = (int)min(max((int64_t)key_lo, base + per * split), (int64_t)key_hi);
-    const int k1 = (int)min((int64_t)key_hi, base + per * (split + 1));
+    const int k1 = split == ns - 1 ? key_hi : (int)min((int64_t)key_hi, base + per * (split + 1));
 
-    // ---- this lane's row ---------------------------------------------------------------------------------------------------
-    const int64_t r = r0 + wave * 16 + l16;
-    const bool row_ok = r < R;
-    const int tok = tok0 + (row_ok ? (int)(r / g) : 0);
-    const int h = hkv * g + (row_ok ? (int)(r % g) : 0);
-    const int b = !prefix ? leader : a.seqstart_q ? interval_of(a.seqstart_q, a.batch, tok) : tok / a.sq;
-    const int first_tok = a.seqstart_q ? a.seqstart_q[b] : b * a.sq;
-    const int sq_b = a.seqstart_q ? a.seqstart_q[b + 1] - first_tok : a.sq;
-    const int i = tok - first_tok;
-    const int sk_b = shared_len(a, b);
-    const MaskYX mk = make_mask(a.mask_type, a.window_left, a.window_right, sq_b, sk_b);
-    const int lo = row_ok ? max(mask_lo(mk, i), k0) : 0;
-    const int hi = row_ok ? min(mask_hi(mk, i, sk_b), k1) : 0;
-    ArithMod amod;
-    if constexpr (kMod) amod.init(a.mod, b, h, i, sq_b, sk_b, a.mask_type, a.window_left, a.window_right);
-    // place of the row's partial result
-    const int64_t wrow = ((int64_t)(a.seqstart_q ? 0 : b) * a.hq + h) * (a.ns_prefix + a.ns_own) + slot;
-    const int64_t wofs = wrow * a.shape_sq + (a.seqstart_q ? tok : i);
+    const bool wave_rows = r0 + wave * 16 * MB < R;  // uniform per wave
 
-    // keys any row of the workgroup sees
-    if (tid == 0) {
-        range[0] = INT32_MAX;
-        range[1] = 0;
+    // ---- this lane's rows, one per 16-row block -----------------------------------------------------------------------------
+    bool row_ok[MB];
+    int tok[MB], h[MB], lo[MB], hi[MB];
+    int64_t wofs[MB];  // places of the rows' partial results
+    ArithMod amod[MB];
+    const int slots = a.ns_prefix + a.ns_own;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+        const int64_t r = r0 + (wave * MB + mb) * 16 + l16;
+        row_ok[mb] = r < R;
+        tok[mb] = tok0 + (row_ok[mb] ? (int)(r / g) : 0);
+        h[mb] = hkv * g + (row_ok[mb] ? (int)(r % g) : 0);
+        const int b = !prefix ? leader : a.seqstart_q ? interval_of(a.seqstart_q, a.batch, tok[mb]) : tok[mb] / a.sq;
+        const int first_tok = a.seqstart_q ? a.seqstart_q[b] : b * a.sq;
+        const int sq_b = a.seqstart_q ? a.seqstart_q[b + 1] - first_tok : a.sq;
+        const int i = tok[mb] - first_tok;
+        const int sk_b = shared_len(a, b);
+        const MaskYX mk = make_mask(a.mask_type, a.window_left, a.window_right, sq_b, sk_b);
+        lo[mb] = row_ok[mb] ? max(mask_lo(mk, i), k0) : 0;
+        hi[mb] = row_ok[mb] ? min(mask_hi(mk, i, sk_b), k1) : 0;
+        if constexpr (kMod) amod[mb].init(a.mod, b, h[mb], i, sq_b, sk_b, a.mask_type, a.window_left, a.window_right);
+        const int64_t head = (int64_t)(a.seqstart_q ? 0 : b) * a.hq + h[mb];
+        wofs[mb] = (head * slots + slot) * a.shape_sq + (a.seqstart_q ? tok[mb] : i);
+        // a sequence without a shared prefix has no prefix item
+        if (!prefix && split == 0 && key_lo == 0 && row_ok[mb] && kg == 0)
+            for (int e = 0; e < a.ns_prefix; ++e) a.lse_acc[wofs[mb] - (int64_t)(slot - e) * a.shape_sq] = -INFINITY;
     }
-    __syncthreads();
-    if (lo < hi && kg == 0) {
-        atomicMin((int*)&range[0], lo);
-        atomicMin((int*)&range[1], -hi);
+    // Keys the item walks.  A mask can leave out whole tiles at either end; where it can leave out many (a window on the
+    // left, or a diagonal that does not end at the last key) the range that any row of the workgroup sees is found first.
+    int vis_lo = k0, vis_hi = k1;
+    if (a.mask_type != 0 && (a.window_left >= 0 || a.mask_type == 1)) {
+        if (tid == 0) {
+            range[0] = INT32_MAX;
+            range[1] = 0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+            if (lo[mb] < hi[mb] && kg == 0) {
+                atomicMin((int*)&range[0], lo[mb]);
+                atomicMin((int*)&range[1], -hi[mb]);
+            }
+        __syncthreads();
+        vis_lo = range[0];
+        vis_hi = -range[1];
     }
-    __syncthreads();
-    const int vis_lo = range[0], vis_hi = -range[1];
     if (vis_lo >= vis_hi) {  // an empty split, or one that every row's mask leaves out
-        if (row_ok && kg == 0) a.lse_acc[wofs] = -INFINITY;
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb)
+            if (row_ok[mb] && kg == 0) a.lse_acc[wofs[mb]] = -INFINITY;
         return;
     }
     const int t_begin = vis_lo / S::TK;
     const int n = (vis_hi + S::TK - 1) / S::TK - t_begin;
-    const bool wave_rows = r0 + wave * 16 < R;  // uniform
-
-    vec8 qf[S::KT];
-    {
-        const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + ((int64_t)tok * a.hq + h) * dq + kg * 8;
-#pragma unroll
-        for (int t = 0; t < S::KT; ++t) {
-            u32x4_t v = {0u, 0u, 0u, 0u};
-            if (row_ok && (!kPad || t * 32 + kg * 8 < dq)) v = ldg16(qp + t * 32);
-            qf[t] = as_vec8<vec8>(v);
-        }
-    }
-    float m_run = -INFINITY, l_run = 0.f;
-    f32x4_t oacc[S::DB];
-#pragma unroll
-    for (int db = 0; db < S::DB; ++db) oacc[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
     // ---- K/V tiles ----------------------------------------------------------------------------------------------------------
     const int32_t* table = a.block_table + (int64_t)leader * a.block_table_stride;
@@ -240,168 +251,203 @@ __global__ __launch_bounds__(256) void shared_prefix_kernel(const SharedPrefixAr
             vreg[u] = fetch(a.v, cr, chunk, dvs);
         }
     };
-    auto store_tile = [&](int buf) {
+    auto store_tile = [&]() {
 #pragma unroll
         for (int u = 0; u < S::LD; ++u) {
             const int row = (u * 256 + tid) / S::CH, chunk = (u * 256 + tid) % S::CH;
-            *(u32x4_t FCK_LDS*)(lds + buf * S::TILEB + row * S::ROWB + ((chunk ^ (row & 7)) << 4)) = staged(kreg[u]);
-            *(u32x4_t FCK_LDS*)(lds + (2 + buf) * S::TILEB + row * S::ROWB + ((chunk ^ shared_v_swizzle<D>(row)) << 4)) = staged(vreg[u]);
+            *(u32x4_t FCK_LDS*)(lds + row * S::ROWB + ((chunk ^ (row & 7)) << 4)) = staged(kreg[u]);
+            *(u32x4_t FCK_LDS*)(lds + S::TILEB + row * S::ROWB + ((chunk ^ shared_v_swizzle<D>(row)) << 4)) = staged(vreg[u]);
         }
     };
 
+    load_tile(0);
+    vec8 qf[MB][S::KT];
+    float m_run[MB], l_run[MB];
+    f32x4_t oacc[MB][S::DB];
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+        const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + ((int64_t)tok[mb] * a.hq + h[mb]) * dq + kg * 8;
+#pragma unroll
+        for (int t = 0; t < S::KT; ++t) {
+            u32x4_t v = {0u, 0u, 0u, 0u};
+            if (row_ok[mb] && (!kPad || t * 32 + kg * 8 < dq)) v = ldg16(qp + t * 32);
+            qf[mb][t] = as_vec8<vec8>(v);
+        }
+        m_run[mb] = -INFINITY;
+        l_run[mb] = 0.f;
+#pragma unroll
+        for (int db = 0; db < S::DB; ++db) oacc[mb][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
     const int tr_key = kg * 4 + (l16 >> 2);
     const int tr_sw = shared_v_swizzle<D>(tr_key);
-    const int tr_base = tr_key * S::ROWB + ((l16 & 2) << 3) + ((l16 & 1) << 3);
-    auto compute = [&](int c, int buf) {
+    const char FCK_LDS* const kt = lds + l16 * S::ROWB;
+    const char FCK_LDS* const vt = lds + S::TILEB + tr_key * S::ROWB + ((l16 & 2) << 3) + ((l16 & 1) << 3);
+    auto compute = [&](int c) {
         const int kb = (t_begin + c) * S::TK;
-        const char FCK_LDS* kt = lds + buf * S::TILEB + l16 * S::ROWB;
-        const char FCK_LDS* vt = lds + (2 + buf) * S::TILEB + tr_base;
         // S^T[key][row] = K . Q^T
-        float x[4 * S::NBK];
-        float tmax = -INFINITY;
+        f32x4_t s[MB][S::NBK];
 #pragma unroll
         for (int nb = 0; nb < S::NBK; ++nb) {
-            f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int mb = 0; mb < MB; ++mb) s[mb][nb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int t = 0; t < S::KT; ++t) {
                 const u32x4_t kf = *(const u32x4_t FCK_LDS*)(kt + nb * 16 * S::ROWB + (((t * 4 + kg) ^ (l16 & 7)) << 4));
-                acc = T::mfma16(as_vec8<vec8>(kf), qf[t], acc);
-            }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int key = kb + nb * 16 + kg * 4 + j;
-                const bool vis = key >= lo && key < hi;
-                float v;
-                if constexpr (kMod)
-                    v = vis ? amod.score(acc[j], key) : -INFINITY;
-                else
-                    v = vis ? acc[j] * a.scale_log2 : -INFINITY;
-                x[nb * 4 + j] = v;
-                tmax = fmaxf(tmax, v);
+                for (int mb = 0; mb < MB; ++mb) s[mb][nb] = T::mfma16(as_vec8<vec8>(kf), qf[mb][t], s[mb][nb]);
             }
         }
-        tmax = quad16_max(tmax);
-        const float m_new = fmaxf(m_run, tmax);
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = fast_exp2(m_run - m_use);
-        m_run = m_new;
-        float psum = 0.f;
-        uint32_t pk[2 * S::NBK];
+        uint32_t pk[MB][2 * S::NBK];
 #pragma unroll
-        for (int e = 0; e < 2 * S::NBK; ++e) {
-            const float p0 = fast_exp2(x[2 * e] - m_use), p1 = fast_exp2(x[2 * e + 1] - m_use);
-            psum += p0 + p1;
-            // P feeds the 16-bit matrix instructions like K and V do; the row sum keeps the unrounded values
-            pk[e] = T::pack2(p0, p1);
+        for (int mb = 0; mb < MB; ++mb) {
+            // scores stay raw and the scale goes into the exponent's fused multiply-add; modified scores are in the log2 domain
+            const float scale = kMod ? 1.f : a.scale_log2;
+            if constexpr (kMod) {
+#pragma unroll
+                for (int nb = 0; nb < S::NBK; ++nb)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[mb][nb][j] = amod[mb].score(s[mb][nb][j], kb + nb * 16 + kg * 4 + j);
+            }
+            // a row that does not exist (lo = hi = 0) computes along on zeros
+            if (__builtin_amdgcn_ballot_w64(row_ok[mb] && (lo[mb] > kb || hi[mb] < kb + S::TK)) != 0) {
+#pragma unroll
+                for (int nb = 0; nb < S::NBK; ++nb)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int key = kb + nb * 16 + kg * 4 + j;
+                        s[mb][nb][j] = key >= lo[mb] && key < hi[mb] ? s[mb][nb][j] : -INFINITY;
+                    }
+            }
+            float tmax = -INFINITY;
+#pragma unroll
+            for (int nb = 0; nb < S::NBK; ++nb)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) tmax = fmaxf(tmax, s[mb][nb][j]);
+            tmax = quad16_max(tmax) * scale;  // scale > 0
+            const float m_new = fmaxf(m_run[mb], tmax);
+            const float m_use = m_new == -INFINITY ? 0.f : m_new;
+            const float alpha = fast_exp2(m_run[mb] - m_use);
+            m_run[mb] = m_new;
+            float psum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 2 * S::NBK; ++e) {
+                const float p0 = fast_exp2(__builtin_fmaf(s[mb][e >> 1][(e & 1) * 2], scale, -m_use));
+                const float p1 = fast_exp2(__builtin_fmaf(s[mb][e >> 1][(e & 1) * 2 + 1], scale, -m_use));
+                psum += p0 + p1;
+                // P feeds the 16-bit matrix instructions like K and V do; the row sum keeps the unrounded values
+                pk[mb][e] = T::pack2(p0, p1);
+            }
+            l_run[mb] = l_run[mb] * alpha + psum;
+            // the maximum of most tiles moves no row
+            if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {
+#pragma unroll
+                for (int db = 0; db < S::DB; ++db) oacc[mb][db] *= alpha;
+            }
         }
-        l_run = l_run * alpha + psum;
-#pragma unroll
-        for (int db = 0; db < S::DB; ++db) oacc[db] *= alpha;
         // O^T[dv][row] += V^T . P^T
 #pragma unroll
-        for (int kk = 0; kk < S::NBK / 2; ++kk) {
-            const u32x4_t pv = {pk[kk * 4], pk[kk * 4 + 1], pk[kk * 4 + 2], pk[kk * 4 + 3]};
+        for (int kk = 0; kk < S::NBK / 2; ++kk)
 #pragma unroll
             for (int db = 0; db < S::DB; ++db) {
                 const char FCK_LDS* p = vt + kk * 32 * S::ROWB + (((db * 2) ^ tr_sw) << 4);
                 const u32x2_t lo4 = lds_read_tr16(p), hi4 = lds_read_tr16(p + 16 * S::ROWB);
                 const u32x4_t av = {lo4[0], lo4[1], hi4[0], hi4[1]};
-                oacc[db] = T::mfma16(as_vec8<vec8>(av), as_vec8<vec8>(pv), oacc[db]);
+#pragma unroll
+                for (int mb = 0; mb < MB; ++mb) {
+                    const u32x4_t pv = {pk[mb][kk * 4], pk[mb][kk * 4 + 1], pk[mb][kk * 4 + 2], pk[mb][kk * 4 + 3]};
+                    oacc[mb][db] = T::mfma16(as_vec8<vec8>(av), as_vec8<vec8>(pv), oacc[mb][db]);
+                }
             }
-        }
     };
 
-    // tile c is in LDS buffer c % 2 behind the barrier of iteration c; tile c + 1 is in flight meanwhile
-    load_tile(0);
+    // tile c is in LDS between the two barriers of iteration c, tile c + 1 in flight
     for (int c = 0; c < n; ++c) {
-        store_tile(c & 1);
+        store_tile();
         __syncthreads();
         if (c + 1 < n) load_tile(c + 1);
-        if (wave_rows) compute(c, c & 1);
+        if (wave_rows) compute(c);
+        __syncthreads();
     }
 
-    l_run = quad16_sum(l_run);
-    if (!row_ok) return;
-    const float inv = l_run == 0.f ? 0.f : a.v_descale / l_run;
-    float* op = a.o_acc + wofs * dvs + kg * 4;
 #pragma unroll
-    for (int db = 0; db < S::DB; ++db) {
-        if (kPad && db * 16 + kg * 4 >= dvs) continue;
-        *reinterpret_cast<f32x4_t*>(op + db * 16) = oacc[db] * inv;
+    for (int mb = 0; mb < MB; ++mb) {
+        l_run[mb] = quad16_sum(l_run[mb]);
+        if (!row_ok[mb]) continue;
+        const float inv = l_run[mb] == 0.f ? 0.f : a.v_descale / l_run[mb];
+        float* op = a.o_acc + wofs[mb] * dvs + kg * 4;
+#pragma unroll
+        for (int db = 0; db < S::DB; ++db) {
+            if (kPad && db * 16 + kg * 4 >= dvs) continue;
+            *reinterpret_cast<f32x4_t*>(op + db * 16) = oacc[mb][db] * inv;
+        }
+        if (kg == 0) a.lse_acc[wofs[mb]] = l_run[mb] == 0.f ? -INFINITY : (m_run[mb] + fast_log2(l_run[mb])) * kLn2;
     }
-    if (kg == 0) a.lse_acc[wofs] = l_run == 0.f ? -INFINITY : (m_run + fast_log2(l_run)) * kLn2;
 }
 
-// Merge of a row's partial results: the prefix splits if its sequence has a shared prefix, the own splits if it has keys
-// behind it.  Dv/4 lanes per row, 4 columns each.
-template <typename T, int DV>
-__global__ __launch_bounds__(256) void shared_prefix_combine_kernel(const SharedPrefixArgs a)
+// Merge of a row's partial results.  Dv/4 lanes per row, 4 columns each; the work is a chain of round trips, so the rows are
+// spread over one-wave workgroups while there are few.
+template <typename T, int DV, int NT>
+__global__ __launch_bounds__(NT) void shared_prefix_combine_kernel(const SharedPrefixArgs a)
 {
     constexpr int TPR = DV / 4;
-    const int64_t item = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;  // (row, head)
+    const int64_t item = (int64_t)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;  // (row, head)
     const int c = threadIdx.x % TPR * 4;
     const int64_t rows = a.seqstart_q ? a.shape_sq : (int64_t)a.batch * a.sq;
     if (item >= rows * a.hq || c >= a.dv) return;
     const int tok = (int)(item / a.hq), h = (int)(item % a.hq);
-    int b, i;
-    if (a.seqstart_q) {
-        b = interval_of(a.seqstart_q, a.batch, tok);
-        if (tok >= a.seqstart_q[b + 1] || tok < a.seqstart_q[b]) return;  // a row behind the last sequence stays as it was
-        i = tok;
-    } else {
-        b = tok / a.sq;
-        i = tok - b * a.sq;
-    }
-    const int own = own_begin(a, b), len = shared_len(a, b);
-    const int first = own > 0 ? 0 : a.ns_prefix;
-    const int last = len > own ? a.ns_prefix + a.ns_own : a.ns_prefix;
-    const int64_t w0 = (((int64_t)(a.seqstart_q ? 0 : b) * a.hq + h) * (a.ns_prefix + a.ns_own) + first) * a.shape_sq + i;
-    f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-    if (last > first) acc = combine_splits<DV>(a.lse_acc, a.o_acc, w0, a.shape_sq, last - first, c, a.dv);
+    if (a.seqstart_q && tok >= a.seqstart_q[a.batch]) return;  // a row behind the last sequence stays as it was
+    const int b = a.seqstart_q ? 0 : tok / a.sq, i = a.seqstart_q ? tok : tok - b * a.sq;
+    const int slots = a.ns_prefix + a.ns_own;
+    const int64_t row = (int64_t)b * a.hq + h, w0 = row * slots * a.shape_sq + i;
+    float lse;
+    const f32x4_t acc = combine_splits<DV>(a.lse_acc, a.o_acc, w0, a.shape_sq, slots, c, a.dv, &lse);
     u32x2_t out;
     out[0] = T::pack2(acc[0], acc[1]);
     out[1] = T::pack2(acc[2], acc[3]);
     *reinterpret_cast<u32x2_t*>(reinterpret_cast<uint16_t*>(a.o) + item * a.dv + c) = out;
-    if (a.lse && c == 0)
-        a.lse[((int64_t)(a.seqstart_q ? 0 : b) * a.hq + h) * a.shape_sq + i] = combine_lse(a.lse_acc, w0, a.shape_sq, last - first);
+    if (a.lse && c == 0) a.lse[row * a.shape_sq + i] = lse;
 }
 
-template <typename T, int D>
+template <typename T, int D, int MB>
 hipError_t launch_general(const SharedPrefixArgs& a, bool uniform, int64_t grid, hipStream_t st)
 {
-    constexpr size_t lds = (size_t)4 * SharedShape<D>::TILEB + 16;
+    constexpr size_t lds = (size_t)2 * SharedShape<D, MB>::TILEB + 16;
     const dim3 blocks((unsigned)grid), threads(256);
     if (a.kv8) {
-        if (uniform) return launch_with_lds<shared_prefix_kernel<T, D, true, true, false, true>>(blocks, threads, lds, st, a);
-        return launch_with_lds<shared_prefix_kernel<T, D, false, true, false, true>>(blocks, threads, lds, st, a);
+        if (uniform) return launch_with_lds<shared_prefix_kernel<T, D, MB, true, true, false, true>>(blocks, threads, lds, st, a);
+        return launch_with_lds<shared_prefix_kernel<T, D, MB, false, true, false, true>>(blocks, threads, lds, st, a);
     }
     if (a.d != D || a.dv != D) {
-        if (uniform) return launch_with_lds<shared_prefix_kernel<T, D, true, true, true, false>>(blocks, threads, lds, st, a);
-        return launch_with_lds<shared_prefix_kernel<T, D, false, true, true, false>>(blocks, threads, lds, st, a);
+        if (uniform) return launch_with_lds<shared_prefix_kernel<T, D, MB, true, true, true, false>>(blocks, threads, lds, st, a);
+        return launch_with_lds<shared_prefix_kernel<T, D, MB, false, true, true, false>>(blocks, threads, lds, st, a);
     }
     if (a.mod.active()) {
-        if (uniform) return launch_with_lds<shared_prefix_kernel<T, D, true, true, false, false>>(blocks, threads, lds, st, a);
-        return launch_with_lds<shared_prefix_kernel<T, D, false, true, false, false>>(blocks, threads, lds, st, a);
+        if (uniform) return launch_with_lds<shared_prefix_kernel<T, D, MB, true, true, false, false>>(blocks, threads, lds, st, a);
+        return launch_with_lds<shared_prefix_kernel<T, D, MB, false, true, false, false>>(blocks, threads, lds, st, a);
     }
-    if (uniform) return launch_with_lds<shared_prefix_kernel<T, D, true, false, false, false>>(blocks, threads, lds, st, a);
-    return launch_with_lds<shared_prefix_kernel<T, D, false, false, false, false>>(blocks, threads, lds, st, a);
+    if (uniform) return launch_with_lds<shared_prefix_kernel<T, D, MB, true, false, false, false>>(blocks, threads, lds, st, a);
+    return launch_with_lds<shared_prefix_kernel<T, D, MB, false, false, false, false>>(blocks, threads, lds, st, a);
 }
 
 template <typename T, int DV>
 hipError_t launch_combine(const SharedPrefixArgs& a, hipStream_t st)
 {
     const int64_t items = (a.seqstart_q ? a.shape_sq : (int64_t)a.batch * a.sq) * a.hq;
-    constexpr int per_wg = 256 / (DV / 4);
-    const int64_t grid = (items + per_wg - 1) / per_wg;
-    if (grid > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((shared_prefix_combine_kernel<T, DV>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    constexpr int per_wg = 256 / (DV / 4), per_wave = 64 / (DV / 4);
+    const int64_t wide = (items + per_wg - 1) / per_wg;
+    if (wide > INT32_MAX) return hipErrorInvalidValue;
+    if (wide < 4 * (int64_t)a.num_cu)
+        hipLaunchKernelGGL((shared_prefix_combine_kernel<T, DV, 64>), dim3((unsigned)((items + per_wave - 1) / per_wave)), dim3(64), 0, st, a);
+    else
+        hipLaunchKernelGGL((shared_prefix_combine_kernel<T, DV, 256>), dim3((unsigned)wide), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
-template <typename T, int D>
-hipError_t launch_d(SharedPrefixArgs& a, int64_t rows_prefix, int64_t rows_own, hipStream_t st)
+template <typename T, int D, int MB>
+hipError_t launch_mb(SharedPrefixArgs& a, int64_t rows_prefix, int64_t rows_own, hipStream_t st)
 {
-    constexpr int BM = SharedShape<D>::BM;
+    constexpr int BM = SharedShape<D, MB>::BM;
     const int64_t p_tiles = (rows_prefix + BM - 1) / BM, o_tiles = (rows_own + BM - 1) / BM;
     const int64_t streams = ((int64_t)a.groups * a.ns_prefix * a.hk + 7) / 8 * 8;
     const int64_t prefix_items = streams * p_tiles;
@@ -411,14 +457,29 @@ hipError_t launch_d(SharedPrefixArgs& a, int64_t rows_prefix, int64_t rows_own, 
     a.own_tiles = (int32_t)o_tiles;
     a.prefix_items = (int32_t)prefix_items;
     // a key tile then never straddles a page
-    const bool uniform = a.page_size % SharedShape<D>::TK == 0;
-    if (hipError_t e = launch_general<T, D>(a, uniform, grid, st); e != hipSuccess) return e;
+    const bool uniform = a.page_size % SharedShape<D, MB>::TK == 0;
+    if (hipError_t e = launch_general<T, D, MB>(a, uniform, grid, st); e != hipSuccess) return e;
     if (a.dv <= 64) return launch_combine<T, 64>(a, st);
     if (a.dv <= 128) return launch_combine<T, 128>(a, st);
     return launch_combine<T, 256>(a, st);
 }
 
+template <typename T, int D>
+hipError_t launch_d(SharedPrefixArgs& a, int64_t rows_prefix, int64_t rows_own, hipStream_t st)
+{
+    if constexpr (D <= 128)
+        if (shared_prefix_blocks(D, rows_prefix) == 2) return launch_mb<T, D, 2>(a, rows_prefix, rows_own, st);
+    return launch_mb<T, D, 1>(a, rows_prefix, rows_own, st);
+}
+
 }  // namespace
+
+int shared_prefix_blocks(int d, int64_t rows_prefix) { return d <= 128 && rows_prefix > 128 ? 2 : 1; }
+
+int shared_prefix_workgroups(int d, int64_t rows_prefix, int num_cu)
+{
+    return (shared_prefix_blocks(d, rows_prefix) == 2 || d == 256 ? 2 : 3) * num_cu;
+}
 
 hipError_t launch_shared_prefix(SharedPrefixArgs a, int d, int dtype, int64_t rows_prefix, int64_t rows_own, hipStream_t st)
 {

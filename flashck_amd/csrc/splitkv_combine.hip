@@ -30,8 +30,9 @@ __global__ __launch_bounds__(NT) void splitkv_combine_kernel(const CombineArgs a
     const int ns = a.num_splits;
     const int64_t w0 = ((b * a.hq + h) * ns) * a.Sq + i;  // split 0; next split is Sq further
 
-    const f32x4_t acc = combine_splits<DV>(a.lse_acc, a.o_acc, w0, a.Sq, ns, c, a.dv);
-    if (a.lse && c == 0) a.lse[(b * a.hq + h) * a.Sq + i] = combine_lse(a.lse_acc, w0, a.Sq, ns);
+    float lse;
+    const f32x4_t acc = combine_splits<DV>(a.lse_acc, a.o_acc, w0, a.Sq, ns, c, a.dv, &lse);
+    if (a.lse && c == 0) a.lse[(b * a.hq + h) * a.Sq + i] = lse;
     if constexpr (std::is_same<T, FP8Out>::value) {
         *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(a.o) + (row * a.hq + h) * a.dv + c) =
             pack_fp8x4_sat(acc[0] * a.o_scale, acc[1] * a.o_scale, acc[2] * a.o_scale, acc[3] * a.o_scale);

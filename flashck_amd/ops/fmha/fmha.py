@@ -890,12 +890,12 @@ def fmha_decode_step(q, knew, vnew, k_cache, v_cache, seqlen_k, block_table, *, 
     return o, seqlen_new
 
 
-def shared_prefix_splits(batch, num_groups, max_group_size, q_num_heads, kv_num_heads, seqlen_q, max_prefix_len, max_own_len,
-                         num_cu=0) -> Tuple[int, int]:
+def shared_prefix_splits(batch, num_groups, max_group_size, q_num_heads, kv_num_heads, seqlen_q, head_dim, max_prefix_len,
+                         max_own_len, num_cu=0) -> Tuple[int, int]:
     """(prefix splits, own splits) fmha_decode_shared_prefix takes by default, from the CU count and the key counts."""
     ns = (ctypes.c_int32(), ctypes.c_int32())
-    _call("fck_fmha_shared_prefix_splits", batch, num_groups, max_group_size, q_num_heads, kv_num_heads, seqlen_q, max_prefix_len,
-          max_own_len, num_cu, ctypes.byref(ns[0]), ctypes.byref(ns[1]))
+    _call("fck_fmha_shared_prefix_splits", batch, num_groups, max_group_size, q_num_heads, kv_num_heads, seqlen_q, head_dim,
+          max_prefix_len, max_own_len, num_cu, ctypes.byref(ns[0]), ctypes.byref(ns[1]))
     return ns[0].value, ns[1].value
 
 
@@ -972,10 +972,12 @@ def fmha_decode_shared_prefix(q, k_cache, v_cache, seqlen_k, block_table, prefix
     if capacity == 0:
         raise ValueError("block_table must have at least one page per sequence")
     max_group_size = min(int(max_group_size), B) if max_group_size > 0 else B
+    # bounds of the longest prefix and of the most keys behind one; they steer the splits and nothing else
+    longest = min(max_seqlen_k, capacity) if max_seqlen_k > 0 else capacity
+    prefix = min(max_prefix_len, longest) if max_prefix_len > 0 else longest
+    own = max(longest - prefix, 1) if max_prefix_len > 0 else longest
     if num_prefix_splits <= 0 or num_splits <= 0:
-        longest = max_seqlen_k if max_seqlen_k > 0 else capacity
-        prefix = min(max_prefix_len, longest) if max_prefix_len > 0 else longest
-        ns = shared_prefix_splits(B, G, max_group_size, Hq, Hk, sq_max, prefix, longest - prefix if max_prefix_len > 0 else longest)
+        ns = shared_prefix_splits(B, G, max_group_size, Hq, Hk, sq_max, max(D, Dv), prefix, own)
         num_prefix_splits = num_prefix_splits if num_prefix_splits > 0 else ns[0]
         num_splits = num_splits if num_splits > 0 else ns[1]
     _debug_validate(seqlen_k=seqlen_k, block_table=block_table, num_total_pages=k_cache.shape[0], page_size=page)
@@ -993,7 +995,7 @@ def fmha_decode_shared_prefix(q, k_cache, v_cache, seqlen_k, block_table, prefix
     with _on(q):
         _call("fck_fmha_decode_shared_prefix", _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(o), _ptr(lse), _ptr(lse_acc), _ptr(o_acc),
               _ptr(cu_seqlens_q), _ptr(seqlen_k), _ptr(block_table), _ptr(cu_groups), _ptr(prefix_lens), B, G, max_group_size, sq, Hq,
-              Hk, D, Dv, sq_max, int(num_prefix_splits), int(num_splits), block_table.shape[1], page, _scale(scale, D), wl, wr,
+              Hk, D, Dv, sq_max, int(num_prefix_splits), int(num_splits), prefix, own, block_table.shape[1], page, _scale(scale, D), wl, wr,
               mask_type, _dtype_id(q), at, _stream())
     del keep
     return o

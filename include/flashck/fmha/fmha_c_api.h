@@ -291,6 +291,8 @@ FCK_EXPORT int fck_fmha_fwd_splitkv_combine_lse(const void* lse_acc, const void*
  *   max_group_size  at most this many sequences of a group share (0: batch); the ones behind read all their own keys
  *   seqlen_k_ptr  int32 [B], key counts with the prefix
  *   q, o, lse     as fck_fmha_fwd_splitkv and its combine; seqlen_q carries total_q in group mode; lse may be NULL
+ *   max_prefix_len, max_own_len  the longest prefix and the most keys a sequence has behind it (0: what the table can address):
+ *                 a split holds ceil(bound / splits) keys rounded up to 64, the last one whatever lies behind the bound
  *   o_acc, lse_acc  fp32 workspace [Bs, Hq, num_prefix_splits + num_own_splits, Sq, Dv] and without Dv
  *                 (fck_fmha_splitkv_workspace_bytes); split counts in [1, 64], fck_fmha_shared_prefix_splits chooses them
  * attrs: ALiBi, soft cap, kv_dtype with its scales.  Two launches.  A row whose mask leaves no key gets zeros and lse -inf;
@@ -303,17 +305,17 @@ FCK_EXPORT int fck_fmha_decode_shared_prefix(const void* q, const void* k_cache,
                                              int64_t num_groups, int64_t max_group_size, int64_t seqlen_q,
                                              int64_t q_num_heads, int64_t kv_num_heads, int64_t qk_head_dim,
                                              int64_t v_head_dim, int64_t q_max_seq_len, int64_t num_prefix_splits,
-                                             int64_t num_own_splits, int64_t batch_stride_block_table,
-                                             int64_t page_block_size, float scale, int64_t window_left,
+                                             int64_t num_own_splits, int64_t max_prefix_len, int64_t max_own_len,
+                                             int64_t batch_stride_block_table, int64_t page_block_size, float scale, int64_t window_left,
                                              int64_t window_right, uint32_t mask_type, int32_t dtype,
                                              const fck_fmha_attrs* attrs, void* stream);
 
 /* Split counts for fck_fmha_decode_shared_prefix from the CU count (num_cu <= 0: of the current device) and the longest
  * prefix and the most keys a sequence has behind it. */
 FCK_EXPORT int fck_fmha_shared_prefix_splits(int64_t batch, int64_t num_groups, int64_t max_group_size, int64_t q_num_heads,
-                                             int64_t kv_num_heads, int64_t seqlen_q, int64_t max_prefix_len,
-                                             int64_t max_own_len, int64_t num_cu, int32_t* prefix_splits,
-                                             int32_t* own_splits);
+                                             int64_t kv_num_heads, int64_t seqlen_q, int64_t head_dim,
+                                             int64_t max_prefix_len, int64_t max_own_len, int64_t num_cu,
+                                             int32_t* prefix_splits, int32_t* own_splits);
 
 /*
  * Attention weight every key receives:
