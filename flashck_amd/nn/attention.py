@@ -102,32 +102,58 @@ class PagedAttention(torch.nn.Module):
             raise ValueError(f"v_cache must be [pages, page_size, {self.kv_num_heads}, {self.v_head_dim}], got {tuple(v_cache.shape)}")
 
     def prefill(self, q, k_cache, v_cache, cu_seqlens_q, *, kv_indptr=None, kv_page_indices=None, kv_last_page_lens=None,
-                seqlen_k=None, block_table=None, max_seqlen_q: int = 0):
+                seqlen_k=None, block_table=None, max_seqlen_q: int = 0, lse=None):
         """Varlen causal attention of packed prompts q [total_q, Hq, D]; K/V addressed by a page list
-        (kv_indptr / kv_page_indices / kv_last_page_lens) or by a block table with seqlen_k."""
+        (kv_indptr / kv_page_indices / kv_last_page_lens) or by a block table with seqlen_k.  lse (fp32 [Hq, total_q],
+        optional) receives the log-sum-exp of every row, for `key_weights`."""
         self._check_cache(q, k_cache, v_cache)
         window = (self.window_left, 0)
+        extra = {} if lse is None else {"lse": lse}
         if kv_indptr is not None:
             return fmha.fmha_batch_prefill(q, k_cache, v_cache, cu_seqlens_q, kv_indptr, kv_page_indices, kv_last_page_lens,
                                            max_seqlen_q=max_seqlen_q, scale=self.scale, mask_type=fmha.MASK_BOTTOM_RIGHT,
-                                           window=window, k_descale=self.k_descale, v_descale=self.v_descale)
+                                           window=window, k_descale=self.k_descale, v_descale=self.v_descale, **extra)
         if block_table is None or seqlen_k is None:
             raise ValueError("prefill needs either kv_indptr/kv_page_indices or block_table/seqlen_k")
         return fmha.fmha_fwd_pagedkv(q, k_cache, v_cache, seqlen_k, block_table, cu_seqlens_q=cu_seqlens_q,
                                      max_seqlen_q=max_seqlen_q, scale=self.scale, mask_type=fmha.MASK_BOTTOM_RIGHT,
-                                     window=window, k_descale=self.k_descale, v_descale=self.v_descale)
+                                     window=window, k_descale=self.k_descale, v_descale=self.v_descale, **extra)
 
     def decode_step(self, q, knew, vnew, k_cache, v_cache, seqlen_k, block_table, *, cu_seqlens_knew=None,
-                    max_seqlen_knew: int = 0, rotary_cos=None, rotary_sin=None, max_seqlen_k: int = 0, out=None):
-        """Append knew/vnew behind seqlen_k[b] tokens (rotating knew and q), attend from the new tokens.
+                    max_seqlen_knew: int = 0, rotary_cos=None, rotary_sin=None, max_seqlen_k: int = 0, out=None,
+                    prefix_lens=None, cu_groups=None, max_group_size: int = 0, max_prefix_len: int = 0, lse=None):
+        """Append knew/vnew behind seqlen_k[b] tokens (rotating knew and q), attend from the new tokens; prefixes that the
+        sequences share (prefix_lens, cu_groups) are read once per group.
         Returns (o, seqlen_k_new); see `fmha_decode_step`."""
         self._check_cache(q, k_cache, v_cache)
+        extra = {} if lse is None else {"lse": lse}
+        if prefix_lens is not None:
+            extra.update(prefix_lens=prefix_lens, cu_groups=cu_groups, max_group_size=max_group_size, max_prefix_len=max_prefix_len)
         return fmha.fmha_decode_step(q, knew, vnew, k_cache, v_cache, seqlen_k, block_table,
                                      cu_seqlens_knew=cu_seqlens_knew, max_seqlen_knew=max_seqlen_knew,
                                      rotary_cos=rotary_cos, rotary_sin=rotary_sin, rope_mode=self.rope_mode,
                                      num_splits=self.num_splits, max_seqlen_k=max_seqlen_k, scale=self.scale,
                                      window_left=self.window_left, workspace=self.workspace, out=out,
-                                     k_descale=self.k_descale, v_descale=self.v_descale)
+                                     k_descale=self.k_descale, v_descale=self.v_descale, **extra)
+
+    def key_weights(self, q, k_cache, lse, seqlen_k, block_table, *, weights=None, cu_seqlens_q=None, max_seqlen_q: int = 0, out=None):
+        """Attention weight the keys of the cache receive from the queries q (rotated, as the attention saw them) whose
+        log-sum-exp `prefill` or `decode_step` left in lse; see `fmha_key_weights`.  Returns fp32 [B, Hk, cols]."""
+        if q.shape[-2] != self.q_num_heads or q.shape[-1] != self.qk_head_dim:
+            raise ValueError(f"q has heads x dim {tuple(q.shape[-2:])}, module expects ({self.q_num_heads}, {self.qk_head_dim})")
+        return fmha.fmha_key_weights(q, k_cache, lse, seqlen_k, block_table, weights=weights, cu_seqlens_q=cu_seqlens_q,
+                                     max_seqlen_q=max_seqlen_q, scale=self.scale, mask_type=fmha.MASK_BOTTOM_RIGHT,
+                                     window=(self.window_left, 0), k_descale=self.k_descale, out=out)
+
+    def evict(self, k_cache, v_cache, weights, seqlen_k, block_table, new_block_table, *, budget: int, recent: int = 0, sinks: int = 0,
+              **outputs):
+        """Keep the `budget` keys of every (sequence, KV head) that received the most weight and move them to new pages; see
+        `fmha_cache_evict`.  Not with a sliding window: evicted keys have no positions.
+        Returns (seqlen_k_new, kept, weights_new)."""
+        if self.window_left >= 0:
+            raise ValueError("a cache read through a sliding window cannot be evicted from: its keys lose their positions")
+        return fmha.fmha_cache_evict(k_cache, v_cache, weights, seqlen_k, block_table, new_block_table, budget=budget, recent=recent,
+                                     sinks=sinks, **outputs)
 
     def extra_repr(self) -> str:
         return (f"q_num_heads={self.q_num_heads}, kv_num_heads={self.kv_num_heads}, qk_head_dim={self.qk_head_dim}, "

@@ -13,6 +13,7 @@ Tensor conventions (T = torch.float16 | torch.bfloat16, contiguous, on the GPU):
 """
 import contextlib
 import ctypes
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -101,7 +102,8 @@ def _ptr(t):
 
 
 def _stream():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # the handle alone: building a torch.cuda.Stream object costs as much as the rest of a small call's host side
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def _call(name, *args):
@@ -824,7 +826,8 @@ class DecodeWorkspace:
 def fmha_decode_step(q, knew, vnew, k_cache, v_cache, seqlen_k, block_table, *, cu_seqlens_knew=None,
                      max_seqlen_knew: int = 0, rotary_cos=None, rotary_sin=None, rope_mode: int = ROPE_NONE,
                      num_splits: int = 0, max_seqlen_k: int = 0, scale: float = 0.0, window_left: int = -1,
-                     workspace: Optional[DecodeWorkspace] = None, out=None, k_descale: float = 1.0, v_descale: float = 1.0):
+                     workspace: Optional[DecodeWorkspace] = None, out=None, k_descale: float = 1.0, v_descale: float = 1.0,
+                     prefix_lens=None, cu_groups=None, max_group_size: int = 0, max_prefix_len: int = 0, lse=None):
     """One serving step over a paged cache: append the new tokens, then attend from them.
 
     The caller side of the split-KV path, FmhaKind::FwdAppendKV -> FwdSplitKV -> FwdSplitKVCombine
@@ -837,6 +840,9 @@ def fmha_decode_step(q, knew, vnew, k_cache, v_cache, seqlen_k, block_table, *, 
          its own position (bottom-right causal; window_left >= 0 adds a sliding window) - and the LSE combine.
     q/knew/vnew are [B, n, H, D] (n new tokens everywhere) or packed [total_new, H, D] with cu_seqlens_knew and
     max_seqlen_knew.  Nothing is read back from the GPU, so a step only enqueues work on the current stream.
+    prefix_lens (with cu_groups, max_group_size, max_prefix_len: see fmha_decode_shared_prefix): the sequences share
+    prefixes, and step 3 reads each of them once per group; num_splits is then the split count of the tokens behind them.
+    lse (fp32 [B,Hq,n] or [Hq,total_new], optional) receives the log-sum-exp of every row (what fmha_key_weights takes).
     With torch.float8_e4m3fn caches the new rows are quantised on their way in and dequantised by the attention
     kernel, both with the static scales k_descale / v_descale.
 
@@ -867,6 +873,18 @@ def fmha_decode_step(q, knew, vnew, k_cache, v_cache, seqlen_k, block_table, *, 
         torch.add(seqlen_k, counts, out=seqlen_new)
     else:
         torch.add(seqlen_k, n, out=seqlen_new)
+    # a lone new token sees every key: no mask needed unless a sliding window is asked for
+    if n == 1 and window_left < 0:
+        mask_type, window = MASK_NONE, (-1, -1)
+    else:
+        mask_type, window = MASK_BOTTOM_RIGHT, (int(window_left), 0)
+    if prefix_lens is not None:
+        o = fmha_decode_shared_prefix(q, k_cache, v_cache, seqlen_new, block_table, prefix_lens, cu_groups=cu_groups,
+                                      max_group_size=max_group_size, max_prefix_len=max_prefix_len, max_seqlen_k=max_seqlen_k,
+                                      num_splits=num_splits, cu_seqlens_q=cu_seqlens_knew, max_seqlen_q=n if packed else 0,
+                                      scale=scale, mask_type=mask_type, window=window, k_descale=k_descale, v_descale=v_descale,
+                                      workspace=ws, out=out, lse=lse)
+        return o, seqlen_new
     if num_splits <= 0:
         if max_seqlen_k <= 0:
             max_seqlen_k = block_table.shape[1] * page  # what the block table can address
@@ -874,19 +892,15 @@ def fmha_decode_step(q, knew, vnew, k_cache, v_cache, seqlen_k, block_table, *, 
         decode_variant = _usable_variant(decode_variant, Hq, Hk, n, D, Dv, plain=not kv_fp8, page_size=page)
     else:
         decode_variant = 0
-    # a lone new token sees every key: no mask needed unless a sliding window is asked for
-    if n == 1 and window_left < 0:
-        mask_type, window = MASK_NONE, (-1, -1)
-    else:
-        mask_type, window = MASK_BOTTOM_RIGHT, (int(window_left), 0)
     shape_batch, shape_sq = (1, q.shape[0]) if packed else (B, n)
     o_acc, lse_acc = ws.partials(shape_batch, Hq, num_splits, shape_sq, Dv, q.device)
     fmha_fwd_splitkv(q, k_cache, v_cache, num_splits, seqlen_k=seqlen_new, block_table=block_table,
                      cu_seqlens_q=cu_seqlens_knew, max_seqlen_q=n if packed else 0, scale=scale, mask_type=mask_type,
                      window=window, o_acc=o_acc, lse_acc=lse_acc, decode_variant=decode_variant, k_descale=k_descale,
                      v_descale=v_descale, max_seqlen_k=max_seqlen_k)
+    extra = {} if lse is None else {"lse": lse}
     o = fmha_fwd_splitkv_combine(lse_acc, o_acc, q.dtype, cu_seqlens_q=cu_seqlens_knew, max_seqlen_q=n if packed else 0,
-                                 out=out)
+                                 out=out, **extra)
     return o, seqlen_new
 
 
@@ -899,15 +913,30 @@ def shared_prefix_splits(batch, num_groups, max_group_size, q_num_heads, kv_num_
     return ns[0].value, ns[1].value
 
 
+# The split counts are functions of the shapes and the CU count alone: decided once per shape.
+_shared_prefix_splits = functools.lru_cache(maxsize=1024)(lambda device, *sizes: shared_prefix_splits(*sizes))
+_key_weights_row_splits = functools.lru_cache(maxsize=1024)(
+    lambda device, *sizes: int(_lib.load().fck_fmha_key_weights_row_splits(*sizes, 0)))
+
+
 def _check_same_device(like, **tensors):
+    device = like.device
     for name, t in tensors.items():
-        if t is not None and t.device != like.device:
-            raise ValueError(f"{name} is on {t.device}, the inputs are on {like.device}")
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the inputs are on {device}")
+
+
+_HERE = contextlib.nullcontext()
 
 
 def _on(t):
     """The device of t made current for a launch (the C ABI launches on the current device and its current stream)."""
-    return torch.cuda.device(t.device) if t.is_cuda else contextlib.nullcontext()
+    return torch.cuda.device(t.device) if t.is_cuda and t.device.index != torch.cuda.current_device() else _HERE
+
+
+def _at(t):
+    """Address of an optional tensor, for arguments declared as pointers."""
+    return None if t is None else t.data_ptr()
 
 
 def _cache_dtype(q, cache):
@@ -977,7 +1006,7 @@ def fmha_decode_shared_prefix(q, k_cache, v_cache, seqlen_k, block_table, prefix
     prefix = min(max_prefix_len, longest) if max_prefix_len > 0 else longest
     own = max(longest - prefix, 1) if max_prefix_len > 0 else longest
     if num_prefix_splits <= 0 or num_splits <= 0:
-        ns = shared_prefix_splits(B, G, max_group_size, Hq, Hk, sq_max, max(D, Dv), prefix, own)
+        ns = _shared_prefix_splits(q.device, B, G, max_group_size, Hq, Hk, sq_max, max(D, Dv), prefix, own)
         num_prefix_splits = num_prefix_splits if num_prefix_splits > 0 else ns[0]
         num_splits = num_splits if num_splits > 0 else ns[1]
     _debug_validate(seqlen_k=seqlen_k, block_table=block_table, num_total_pages=k_cache.shape[0], page_size=page)
@@ -986,15 +1015,18 @@ def fmha_decode_shared_prefix(q, k_cache, v_cache, seqlen_k, block_table, prefix
         _check_tensor("lse", lse, dtype=torch.float32)
         _check_shape("lse", lse, (Hq, sq) if group else (B, Hq, sq), q)
     shape_batch, total = (1 if group else B), int(num_prefix_splits) + int(num_splits)
+    rows = shape_batch * Hq * total * sq
     if workspace is not None:
-        o_acc, lse_acc = workspace.partials(shape_batch, Hq, total, sq, Dv, q.device)
-    else:
-        o_acc, lse_acc = splitkv_workspace(shape_batch, Hq, sq, Dv, total, q.device)
+        o_acc, lse_acc = (x.data_ptr() for x in workspace.partials(shape_batch, Hq, total, sq, Dv, q.device))
+    else:  # one buffer: o_acc [Bs,Hq,ns,Sq,Dv] and behind it lse_acc [Bs,Hq,ns,Sq]
+        partials = torch.empty(rows * (Dv + 1), dtype=torch.float32, device=q.device)
+        o_acc = partials.data_ptr()
+        lse_acc = o_acc + rows * Dv * 4
     wl, wr = _window(window)
     at, keep = _attrs(q, None, alibi_slopes, logits_soft_cap, group, B, sq, 1, kv_fp8, k_descale, v_descale)
     with _on(q):
-        _call("fck_fmha_decode_shared_prefix", _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(o), _ptr(lse), _ptr(lse_acc), _ptr(o_acc),
-              _ptr(cu_seqlens_q), _ptr(seqlen_k), _ptr(block_table), _ptr(cu_groups), _ptr(prefix_lens), B, G, max_group_size, sq, Hq,
+        _call("fck_fmha_decode_shared_prefix", _at(q), _at(k_cache), _at(v_cache), _at(o), _at(lse), lse_acc, o_acc,
+              _at(cu_seqlens_q), _at(seqlen_k), _at(block_table), _at(cu_groups), _at(prefix_lens), B, G, max_group_size, sq, Hq,
               Hk, D, Dv, sq_max, int(num_prefix_splits), int(num_splits), prefix, own, block_table.shape[1], page, _scale(scale, D), wl, wr,
               mask_type, _dtype_id(q), at, _stream())
     del keep
@@ -1054,13 +1086,13 @@ def fmha_key_weights(q, k_cache, lse, seqlen_k, block_table=None, *, weights=Non
         _debug_validate(seqlen_k=seqlen_k, block_table=block_table, num_total_pages=k_cache.shape[0], page_size=page)
     o = _out("out", out, (B, Hk, cols), torch.float32, q)
     if num_row_splits <= 0:
-        num_row_splits = int(_lib.load().fck_fmha_key_weights_row_splits(B, Hq, Hk, sq_max, cols, D, mask_type, 0))
+        num_row_splits = _key_weights_row_splits(q.device, B, Hq, Hk, sq_max, cols, D, mask_type)
     partial = torch.empty(num_row_splits, B, Hk, cols, dtype=torch.float32, device=q.device) if num_row_splits > 1 else None
     wl, wr = _window(window)
     at, keep = _attrs(q, None, alibi_slopes, logits_soft_cap, group, B, sq, 1, kv_fp8, k_descale, 1.0)
     with _on(q):
-        _call("fck_fmha_key_weights", _ptr(q), _ptr(k_cache), _ptr(lse), _ptr(weights), _ptr(o), _ptr(partial), _ptr(cu_seqlens_q), _ptr(seqlen_k),
-              _ptr(block_table), stride, page, B, sq, sk, cols, Hq, Hk, D, sq_max, num_row_splits, _scale(scale, D), wl, wr, mask_type, _dtype_id(q),
+        _call("fck_fmha_key_weights", _at(q), _at(k_cache), _at(lse), _at(weights), _at(o), _at(partial), _at(cu_seqlens_q), _at(seqlen_k),
+              _at(block_table), stride, page, B, sq, sk, cols, Hq, Hk, D, sq_max, num_row_splits, _scale(scale, D), wl, wr, mask_type, _dtype_id(q),
               at, _stream())
     del keep
     return o
@@ -1125,8 +1157,8 @@ def fmha_cache_evict(k_cache, v_cache, weights, seqlen_k, block_table, new_block
         validate_paged(seqlen_k=seqlen_k, block_table=block_table, num_total_pages=k_cache.shape[0], page_size=page, check=True)
         _validate_new_pages(seqlen_k, block_table, new_block_table, budget, page, nk, same_pool)
     with _on(k_cache):
-        _call("fck_fmha_cache_evict", _ptr(k_cache), _ptr(v_cache), _ptr(nk), _ptr(nv), _ptr(weights), _ptr(weights_new), _ptr(seqlen_k),
-              _ptr(seqlen_new), _ptr(kept), _ptr(block_table), block_table.shape[1], page, _ptr(new_block_table), new_block_table.shape[1],
+        _call("fck_fmha_cache_evict", _at(k_cache), _at(v_cache), _at(nk), _at(nv), _at(weights), _at(weights_new), _at(seqlen_k),
+              _at(seqlen_new), _at(kept), _at(block_table), block_table.shape[1], page, _at(new_block_table), new_block_table.shape[1],
               nk.shape[1], B, Hk, D, v_cache.shape[3], cols, budget, recent, sinks, _dtype_id(k_cache), _stream())
     return seqlen_new, kept, weights_new
 

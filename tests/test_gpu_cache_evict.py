@@ -164,3 +164,47 @@ def test_the_whole_sequence(fmha):
     assert not got[:, :, budget + 2:].any()
     total = sum(want_w[b, h, torch.tensor(kept_ref[b][h])].sum().item() for b in range(2) for h in range(hk))
     assert abs(got.sum().item() - (total + 2 * 2 * hq)) <= 1e-4 * (total + 2 * 2 * hq)
+
+
+def test_captured_and_replayed(fmha):
+    g = torch.Generator().manual_seed(13)
+    lens = [500, 300]
+    kc, vc, table = (dev(x) for x in lc.pages(g, lens, 16, 2, 64, 64, torch.bfloat16, extra=20))
+    used = set(table.flatten().tolist())
+    free = [p for p in range(kc.shape[0]) if p not in used][:16]
+    new_table = _i32(free).view(2, 8)
+    w, n = torch.rand(2, 2, 500, device="cuda"), _i32(lens)
+    outs = dict(out_seqlen=_i32([0, 0]), out_kept=torch.zeros(2, 2, 128, dtype=torch.int32, device="cuda"), out_weights=torch.zeros_like(w))
+    kw = dict(budget=128, recent=10, sinks=3)
+    fmha.fmha_cache_evict(kc, vc, w, n, table, new_table, **kw, **outs)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        fmha.fmha_cache_evict(kc, vc, w, n, table, new_table, **kw, **outs)
+    for step in range(4):
+        w.copy_(torch.rand_like(w))
+        n.sub_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        got, rows = [x.clone() for x in outs.values()], _bytes(kc).clone()
+        again = fmha.fmha_cache_evict(kc, vc, w, n, table, new_table, **kw)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, again)) and torch.equal(rows, _bytes(kc)), f"replay {step}"
+
+
+def test_on_another_stream(fmha):
+    g = torch.Generator().manual_seed(14)
+    lens = [3000, 2000]
+    kc, vc, table = (dev(x) for x in lc.pages(g, lens, 64, 2, 64, 64, torch.bfloat16))
+    w, n, new_table = torch.rand(2, 2, 3000, device="cuda"), _i32(lens), _i32([3, 0, 5, 1, 7, 2, 4, 6]).view(2, 4)
+    pools = [[torch.zeros(8, 64, 2, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2)] for _ in range(3)]
+    run = lambda p: fmha.fmha_cache_evict(kc, vc, w, n, table, new_table, budget=256, new_k_cache=p[0], new_v_cache=p[1])
+    first = run(pools[0])
+    torch.cuda.synchronize()
+    got = []
+    for p in pools[1:]:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got.append(run(p))
+    torch.cuda.synchronize()
+    for p, x in zip(pools[1:], got):
+        assert all(torch.equal(a, b) for a, b in zip(first, x)) and all(torch.equal(a, b) for a, b in zip(pools[0], p))

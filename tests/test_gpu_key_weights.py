@@ -180,3 +180,41 @@ def test_long_packed_quantised_and_modified_runs(fmha):
                                 max_seqlen_q=270, max_seqlen_k=300, alibi_slopes=dev(slopes), logits_soft_cap=3.0, **kw).cpu()
     want = lc.key_weights(c["q"], c["keys"], c["lse"], 300, 0.125, starts=starts, cap=3.0, slopes=slopes, **kw)
     assert ((out.double() - want).abs() - 2e-4 * want).max() <= 1e-9  # the slopes add up to 75: fp32 steps of 2^-17 there
+
+
+@pytest.mark.parametrize("sq,hq,splits", [(1, 8, 1), (60, 4, 1), (300, 4, 2)])
+def test_captured_and_replayed(fmha, sq, hq, splits):
+    lens, kw = [400, 330], dict(mask_type=2, window=(-1, 0))
+    c = _case(14, lens, sq, hq, 2, 128, torch.bfloat16, 64, **kw)
+    q, lse, n, w = dev(c["q"]), dev(c["lse"]), _i32(lens), torch.zeros(2, 2, 400, device="cuda")
+    args = (q, dev(c["kc"]), lse, n, dev(c["table"]))
+    kw["num_row_splits"] = splits
+    out = torch.empty_like(w)
+    fmha.fmha_key_weights(*args, weights=w, out=out, **kw)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        fmha.fmha_key_weights(*args, weights=w, out=out, **kw)
+    for step in range(4):
+        q.mul_(0.9)
+        n.sub_(3)
+        w.copy_(torch.rand_like(w))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(got, fmha.fmha_key_weights(*args, weights=w, **kw)), f"replay {step}"
+
+
+def test_on_another_stream(fmha):
+    lens, kw = [500, 444], dict(mask_type=2, window=(-1, 0))
+    c = _case(15, lens, 300, 4, 2, 128, torch.bfloat16, 64, **kw)
+    args = (dev(c["q"]), dev(c["kc"]), dev(c["lse"]), _i32(lens), dev(c["table"]))
+    alone = fmha.fmha_key_weights(*args, num_row_splits=2, **kw)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for s in (torch.cuda.Stream(), torch.cuda.Stream()):
+            with torch.cuda.stream(s):
+                got.append(fmha.fmha_key_weights(*args, num_row_splits=2, **kw))
+        torch.cuda.synchronize()
+        assert all(torch.equal(alone, x) for x in got)

@@ -199,3 +199,76 @@ def test_without_an_lse(fmha):
     c = _case(16, [2], [20], [1], 4, 4, 64, torch.float16, 16)
     o, _ = _run(fmha, c, lse=False, cu_groups=None)
     assert (o.double() - lc.decode(c["q"], c["kc"], c["vc"], c["lens"], c["table"], 0.125)[0]).abs().max() <= 2 * U[torch.float16] * 6 + 1e-5
+
+
+def _device_case(c):
+    i32 = lambda x: dev(torch.tensor(x, dtype=torch.int32))
+    return dict(q=dev(c["q"]), k_cache=dev(c["kc"]), v_cache=dev(c["vc"]), seqlen_k=i32(c["lens"]), block_table=dev(c["table"]),
+                prefix_lens=i32(c["prefixes"]), cu_groups=i32(c["starts"]))
+
+
+def test_captured_and_replayed(fmha):
+    c = _case(17, [5, 3], [131, 40], [3, 64, 70], 8, 2, 128, torch.bfloat16, 64)
+    t = _device_case(c)
+    lse = torch.empty(8, 8, 1, device="cuda")
+    out = torch.empty_like(t["q"])
+    fmha.fmha_decode_shared_prefix(**t, out=out, lse=lse)   # warm: the launch opt-ins
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        fmha.fmha_decode_shared_prefix(**t, out=out, lse=lse)
+    g = torch.Generator().manual_seed(18)
+    for step in range(4):
+        t["q"].copy_(lc.randn(g, *t["q"].shape, dtype=torch.bfloat16))
+        t["seqlen_k"].sub_(1)
+        t["prefix_lens"].sub_(1)
+        graph.replay()
+        torch.cuda.synchronize()
+        got, got_lse = out.clone(), lse.clone()
+        eager_lse = torch.empty_like(lse)
+        eager = fmha.fmha_decode_shared_prefix(**t, lse=eager_lse)
+        torch.cuda.synchronize()
+        assert torch.equal(got, eager) and torch.equal(got_lse, eager_lse), f"replay {step}"
+
+
+def test_on_another_stream(fmha):
+    # two calls at once on two streams, each with a workspace of its own, give what they give alone
+    cases = [_case(19 + k, [6], [200], [3, 64, 70], 8, 2, 128, torch.bfloat16, 64) for k in range(2)]
+    inputs = [_device_case(c) for c in cases]
+    alone = [fmha.fmha_decode_shared_prefix(**t) for t in inputs]
+    torch.cuda.synchronize()
+    streams, spaces = [torch.cuda.Stream() for _ in range(2)], [fmha.DecodeWorkspace() for _ in range(2)]
+    for _ in range(5):
+        got = []
+        for t, s, ws in zip(inputs, streams, spaces):
+            with torch.cuda.stream(s):
+                got.append(fmha.fmha_decode_shared_prefix(**t, workspace=ws))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(alone, got))
+
+
+def test_long_cache_offsets(fmha):
+    # pages that lie beyond 2^31 elements and 2^32 bytes of the pools
+    c = _case(21, [3], [130], [5, 64], 8, 8, 128, torch.bfloat16, 128)
+    pages = 17000   # x 128 x 8 x 128 elements = 2.2e9, 4.5 GB
+    n = c["kc"].shape[0]
+    kc = torch.zeros(pages, 128, 8, 128, dtype=torch.bfloat16, device="cuda")
+    vc = torch.zeros_like(kc)
+    kc[pages - n:], vc[pages - n:] = dev(c["kc"]), dev(c["vc"])
+    ref = lc.decode(c["q"], c["kc"], c["vc"], c["lens"], c["table"], 128 ** -0.5)
+    t = _device_case(c)
+    t.update(k_cache=kc, v_cache=vc, block_table=t["block_table"] + (pages - n))
+    lse = torch.empty(3, 8, 1, device="cuda")
+    o = fmha.fmha_decode_shared_prefix(**t, lse=lse)
+    w = fmha.fmha_key_weights(t["q"], kc, lse, t["seqlen_k"], t["block_table"])
+    kept_w, table = torch.rand_like(w), torch.arange(3, dtype=torch.int32, device="cuda").view(3, 1)
+    _, kept, _ = fmha.fmha_cache_evict(kc, vc, kept_w, t["seqlen_k"], t["block_table"], table, budget=100)
+    torch.cuda.synchronize()
+    _check(o.cpu(), lse.cpu(), *ref, torch.bfloat16)
+    assert (w.sum(dim=2).cpu() - 1.0).abs().max() <= 1e-4
+    kept = kept.cpu()
+    for h in (0, 7):
+        for j in (0, 99):
+            p = int(kept[2, h, j])
+            assert torch.equal(kc[2, j, h].cpu(), c["kc"][c["table"][2, p // 128], p % 128, h])
+            assert torch.equal(vc[2, j, h].cpu(), c["vc"][c["table"][2, p // 128], p % 128, h])
