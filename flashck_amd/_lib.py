@@ -44,7 +44,8 @@ SIGNATURES = {
     "fck_fmha_shared_prefix_splits": (ctypes.c_int, [_i64] * 10 + [_vp] * 2),
     "fck_fmha_key_weights_row_splits": (ctypes.c_int, [_i64] * 6 + [_u32, _i64]),
     "fck_fmha_key_weights": (ctypes.c_int, [_vp] * 9 + [_i64] * 11 + [_f32, _i64, _i64, _u32, _i32, _ap, _vp]),
-    "fck_fmha_cache_evict": (ctypes.c_int, [_vp] * 10 + [_i64] * 2 + [_vp] + [_i64] * 10 + [_i32, _vp]),
+    "fck_fmha_cache_evict_workspace_bytes": (ctypes.c_size_t, [_i64] * 4),
+    "fck_fmha_cache_evict": (ctypes.c_int, [_vp] * 11 + [_i64] * 2 + [_vp] + [_i64] * 10 + [_i32, _vp]),
     "fck_fmha_fwd_appendkv": (ctypes.c_int, [_vp] * 7 + [_i64, _vp, _vp, _i64, _i32, _i32, _vp, _i64, _i64, _vp]
                               + [_i64] * 6 + [_i32, _vp]),
     "fck_fmha_fwd_appendkv_attrs": (ctypes.c_int, [_vp] * 7 + [_i64, _vp, _vp, _i64, _i32, _i32, _vp, _i64, _i64, _vp]

@@ -13,6 +13,10 @@
 namespace fck {
 namespace {
 
+constexpr int kEvictParts = 8;           // workgroups per row of the wide choice
+// columns from which it is taken: one sequence, 8 heads, choice and move, with one and with 8 workgroups per row: 45 and 49 us
+// at 32768 keys, 90 and 49 us at 131072
+constexpr int64_t kEvictWideCols = 65536;
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
 
@@ -27,48 +31,78 @@ __device__ __forceinline__ uint32_t weight_key(float w)
 // The histogram of one digit: kBins counters in kColumns copies, a lane adds to copy lane % kColumns.
 constexpr int kBits = 11, kBins = 1 << kBits, kColumns = 8;
 
-// One workgroup per (sequence, KV head); bound by the walks over its weights (L2 round trips), so they are few and wide: a wave
-// owns a contiguous sixteenth of the row and reads 4 weights per lane and load.
+// The choice of one (sequence, KV head), by `parts` workgroups of 16 waves.  Bound by the walks over its weights (L2 round
+// trips and some 20 instructions per weight), so they are few and wide: a wave owns a contiguous part of the row and reads 4
+// weights per lane and load.
 //   1. The want-th largest key of the middle, 11 bits per walk, from a histogram in LDS with a copy for every 8th lane, so
 //      that equal weights, zeros above all, meet at an address seldom (one copy and 8 bits per walk: 369 us for a sequence of
-//      131072 keys and 8 heads; a copy per lane: 154 us).
+//      131072 keys and 8 heads; a copy per lane: 154 us; so: 107 us).
 //   2. A walk that counts what each wave keeps, and one that writes it from the wave's first rank on: ranks are ballots, and
 //      no barrier lies inside a walk.
-__global__ __launch_bounds__(kThreads) void evict_select_kernel(const CacheEvictArgs a)
-{
-    __shared__ int hist[kBins * kColumns];  // [digit][copy]
-    __shared__ __align__(16) int digits[kBins], groups[kBins / 64];
-    __shared__ int chosen[3];
-    __shared__ int counts[2][kWaves];
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int hkv = blockIdx.x % a.hk, b = blockIdx.x / a.hk;
-    const int64_t cap = (int64_t)a.block_table_stride * a.page_size;
-    const int len = __builtin_amdgcn_readfirstlane((int)min((int64_t)max(a.seqlen_k[b], 0), cap));
-    const int n_keep = min(len, a.budget);
-    const float* const w = a.weights + ((int64_t)b * a.hk + hkv) * a.cols;
-    float* const nw = a.new_weights + ((int64_t)b * a.hk + hkv) * a.cols;
-    int32_t* const kept = a.kept + ((int64_t)b * a.hk + hkv) * a.budget;
-    const bool vec = a.cols % 4 == 0 && (reinterpret_cast<uintptr_t>(a.weights) & 15) == 0;
+struct SelectLds {
+    int hist[kBins * kColumns];  // [digit][copy]
+    __align__(16) int digits[kBins];
+    int groups[kBins / 64];
+    int chosen[3];
+    int counts[2][kWaves];
+};
 
-    // positions [0, lo) and [hi, len) are kept anyway, `want` of [lo, hi) by weight
-    const bool all = len <= a.budget;
-    const int lo = all ? len : a.sinks, hi = all ? len : len - a.recent;
-    const int want = all ? 0 : a.budget - a.sinks - a.recent;
+struct Select {
+    const CacheEvictArgs& a;
+    SelectLds& lds;
+    int tid, lane, wave, hkv, b, part, parts;
+    int len, n_keep, lo, hi, want, seg0, seg1;
+    bool all, vec;
+    const float* w;
+    float* nw;
+    int32_t* kept;
+    // the want-th largest key in the digits of `mask`, and how many of the positions whose key equals it are kept
+    uint32_t threshold = 0, mask = 0;
+    int left = 0;
 
-    const int seg = ((len + kWaves - 1) / kWaves + 255) / 256 * 256;
-    const int seg0 = (int)min((int64_t)wave * seg, (int64_t)len), seg1 = (int)min((int64_t)(wave + 1) * seg, (int64_t)len);
+    __device__ __forceinline__ Select(const CacheEvictArgs& a_, SelectLds& lds_, int row, int part_, int parts_) : a(a_), lds(lds_)
+    {
+        tid = threadIdx.x;
+        lane = tid & 63;
+        wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        hkv = row % a.hk;
+        b = row / a.hk;
+        part = part_;
+        parts = parts_;
+        const int64_t cap = (int64_t)a.block_table_stride * a.page_size;
+        len = __builtin_amdgcn_readfirstlane((int)min((int64_t)max(a.seqlen_k[b], 0), cap));
+        n_keep = min(len, a.budget);
+        w = a.weights + (int64_t)row * a.cols;
+        nw = a.new_weights + (int64_t)row * a.cols;
+        kept = a.kept + (int64_t)row * a.budget;
+        vec = a.cols % 4 == 0 && (reinterpret_cast<uintptr_t>(a.weights) & 15) == 0;
+        // positions [0, lo) and [hi, len) are kept anyway, `want` of [lo, hi) by weight
+        all = len <= a.budget;
+        lo = all ? len : a.sinks;
+        hi = all ? len : len - a.recent;
+        want = all ? 0 : a.budget - a.sinks - a.recent;
+        left = want;
+        const int waves = parts * kWaves;
+        const int64_t seg = ((len + waves - 1) / waves + 255) / 256 * 256;
+        seg0 = (int)min((part * kWaves + wave) * seg, (int64_t)len);
+        seg1 = (int)min((part * kWaves + wave + 1) * seg, (int64_t)len);
+    }
+
     // the 4 weights from position t on; a position the weights have no column for has received nothing
-    auto load4 = [&](int t) -> f32x4_t {
+    __device__ __forceinline__ f32x4_t load4(int t) const
+    {
         if (vec && t + 4 <= a.cols) return *reinterpret_cast<const f32x4_t*>(w + t);
         f32x4_t x;
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = t + e < a.cols ? w[t + e] : 0.f;
         return x;
-    };
+    }
+
     // calls f(position of the lane's first weight, its 4 weights, whether all of the wave's 256 lie in the middle) for the
-    // wave's segment; other positions may lie behind the row, which is f's to leave out.  Four loads are in flight per lane.
-    auto walk = [&](auto f) {
+    // wave's part; other positions may lie behind the row, which is f's to leave out.  Four loads are in flight per lane.
+    template <typename F>
+    __device__ __forceinline__ void walk(F f) const
+    {
         auto call = [&](int t0, const f32x4_t& x) {
             if (t0 >= lo && t0 + 256 <= hi)
                 f(t0 + lane * 4, x, std::true_type{});
@@ -84,96 +118,101 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(const CacheEvict
             for (int u = 0; u < 4; ++u) call(t0 + u * 256, x[u]);
         }
         for (; t0 < seg1; t0 += 256) call(t0, load4(t0 + lane * 4));
-    };
+    }
 
-    uint32_t threshold = 0;  // the want-th largest key, in the digits that decide
-    int equal_wanted = 0;    // how many of the positions whose key equals it are kept
-    if (want > 0) {
-        uint32_t mask = 0;
-        int left = want;
-        for (int shift = 32 - kBits; mask != 0xffffffffu; shift = max(shift - kBits, 0)) {
-            const uint32_t digit_mask = (kBins - 1u) << shift & ~mask;
-            for (int e = tid; e < kBins * kColumns; e += kThreads) hist[e] = 0;
-            __syncthreads();
-            walk([&](int t, const f32x4_t& x, auto middle) {
+    __device__ __forceinline__ static int shift_of(int digit) { return max(32 - kBits * (digit + 1), 0); }
+    __device__ __forceinline__ uint32_t digit_bits(int digit) const { return (kBins - 1u) << shift_of(digit) & ~mask; }
+
+    // counts the digit of the keys that begin like the threshold: lds.digits
+    __device__ __forceinline__ void histogram(int digit)
+    {
+        const int shift = shift_of(digit);
+        const uint32_t bits = digit_bits(digit);
+        for (int e = tid; e < kBins * kColumns; e += kThreads) lds.hist[e] = 0;
+        __syncthreads();
+        walk([&](int t, const f32x4_t& x, auto middle) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t key = weight_key(x[e]);
-                    const bool in = decltype(middle)::value || (t + e >= lo && t + e < hi);
-                    if (in && (key & mask) == threshold) atomicAdd(&hist[((key & digit_mask) >> shift) * kColumns + lane % kColumns], 1);
-                }
-            });
-            __syncthreads();
-            // the digit of the left-th largest: by groups of 64 digits first
-            for (int d = tid; d < kBins; d += kThreads) {
-                int sum = 0;
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t key = weight_key(x[e]);
+                const bool in = decltype(middle)::value || (t + e >= lo && t + e < hi);
+                if (in && (key & mask) == threshold) atomicAdd(&lds.hist[((key & bits) >> shift) * kColumns + lane % kColumns], 1);
+            }
+        });
+        __syncthreads();
+        for (int d = tid; d < kBins; d += kThreads) {
+            int sum = 0;
 #pragma unroll
-                for (int c = 0; c < kColumns; ++c) sum += hist[d * kColumns + ((c + d) & (kColumns - 1))];
-                digits[d] = sum;
-            }
-            __syncthreads();
-            if (tid < kBins / 64) {
-                int sum = 0;
-                for (int d = 0; d < 64; ++d) sum += digits[tid * 64 + ((d + tid) & 63)];
-                groups[tid] = sum;
-            }
-            __syncthreads();
-            if (tid < kBins / 64) {
-                int above = 0;
-                for (int j = 0; j < kBins / 64; ++j) above += j > tid ? groups[j] : 0;
-                if (above < left && left <= above + groups[tid]) {  // exactly one thread
-                    chosen[0] = tid * 64;
-                    chosen[1] = left - above;
-                }
-            }
-            __syncthreads();
-            const int first = chosen[0], in_group = chosen[1];
-            __syncthreads();
-            if (tid < 64) {
-                int above = 0;
-                for (int j = 0; j < 64; j += 4) {
-                    const u32x4_t n = *reinterpret_cast<const u32x4_t*>(&digits[first + j]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) above += j + e > tid ? (int)n[e] : 0;
-                }
-                const int here = digits[first + tid];
-                if (above < in_group && in_group <= above + here) {  // exactly one thread
-                    chosen[0] = first + tid;
-                    chosen[1] = in_group - above;
-                    chosen[2] = here;
-                }
-            }
-            __syncthreads();
-            threshold |= (uint32_t)chosen[0] << shift;
-            left = chosen[1];
-            mask |= digit_mask;
-            if (chosen[2] == left) break;  // every key that begins like this is kept: the digits behind do not matter
-            __syncthreads();
+            for (int c = 0; c < kColumns; ++c) sum += lds.hist[d * kColumns + ((c + d) & (kColumns - 1))];
+            lds.digits[d] = sum;
         }
-        equal_wanted = left;
-        const uint32_t m = mask;
-        int sure = 0, equal = 0;
+        __syncthreads();
+    }
+
+    // the digit of the left-th largest from lds.digits, by groups of 64 digits first; true when no further digit matters
+    __device__ __forceinline__ bool take_digit(int digit)
+    {
+        if (tid < kBins / 64) {
+            int sum = 0;
+            for (int d = 0; d < 64; ++d) sum += lds.digits[tid * 64 + ((d + tid) & 63)];
+            lds.groups[tid] = sum;
+        }
+        __syncthreads();
+        if (tid < kBins / 64) {
+            int above = 0;
+            for (int j = 0; j < kBins / 64; ++j) above += j > tid ? lds.groups[j] : 0;
+            if (above < left && left <= above + lds.groups[tid]) {  // exactly one thread
+                lds.chosen[0] = tid * 64;
+                lds.chosen[1] = left - above;
+            }
+        }
+        __syncthreads();
+        const int first = lds.chosen[0], in_group = lds.chosen[1];
+        __syncthreads();
+        if (tid < 64) {
+            int above = 0;
+            for (int j = 0; j < 64; j += 4) {
+                const u32x4_t n = *reinterpret_cast<const u32x4_t*>(&lds.digits[first + j]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) above += j + e > tid ? (int)n[e] : 0;
+            }
+            const int here = lds.digits[first + tid];
+            if (above < in_group && in_group <= above + here) {  // exactly one thread
+                lds.chosen[0] = first + tid;
+                lds.chosen[1] = in_group - above;
+                lds.chosen[2] = here;
+            }
+        }
+        __syncthreads();
+        const uint32_t bits = digit_bits(digit);
+        threshold |= (uint32_t)lds.chosen[0] << shift_of(digit);
+        left = lds.chosen[1];
+        mask |= bits;
+        const bool done = mask == 0xffffffffu || lds.chosen[2] == left;  // every key that begins like this is kept
+        __syncthreads();
+        return done;
+    }
+
+    // (kept without question, equal to the threshold) of the wave's part
+    __device__ __forceinline__ void count(int& sure, int& equal) const
+    {
+        int s = 0, q = 0;
         walk([&](int t, const f32x4_t& x, auto in) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int p = t + e;
-                const uint32_t key = weight_key(x[e]) & m;
+                const uint32_t key = weight_key(x[e]) & mask;
                 const bool middle = decltype(in)::value || (p >= lo && p < hi);
-                sure += __builtin_popcountll(__builtin_amdgcn_ballot_w64(p < len && (!middle || key > threshold)));
-                equal += __builtin_popcountll(__builtin_amdgcn_ballot_w64(middle && key == threshold));
+                s += __builtin_popcountll(__builtin_amdgcn_ballot_w64(p < len && (!middle || key > threshold)));
+                q += __builtin_popcountll(__builtin_amdgcn_ballot_w64(middle && key == threshold));
             }
         });
-        if (lane == 0) {
-            counts[0][wave] = sure;
-            counts[1][wave] = equal;
-        }
-        __syncthreads();
-        int rank = 0, equal_left = equal_wanted;
-        for (int v = 0; v < wave; ++v) {
-            const int eq = min(counts[1][v], equal_left);
-            rank += counts[0][v] + eq;
-            equal_left -= eq;
-        }
+        sure = s;
+        equal = q;
+    }
+
+    // writes what the wave's part keeps from `rank` on; equal_left of the keys that equal the threshold are still wanted
+    __device__ __forceinline__ void write(int rank, int equal_left) const
+    {
         walk([&](int t, const f32x4_t& x, auto in) {
             // per element: kept without question, or equal to the threshold and early enough
             uint64_t keep_mask[4], eq_mask[4];
@@ -181,7 +220,7 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(const CacheEvict
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int p = t + e;
-                const uint32_t key = weight_key(x[e]) & m;
+                const uint32_t key = weight_key(x[e]) & mask;
                 const bool middle = decltype(in)::value || (p >= lo && p < hi);
                 mine[e] = p < len && (!middle || key > threshold);
                 eq[e] = middle && key == threshold;
@@ -218,22 +257,137 @@ __global__ __launch_bounds__(kThreads) void evict_select_kernel(const CacheEvict
                     ++at;
                 }
         });
-    } else {
-        // all of them, or the sinks and the most recent ones
-        for (int j = tid; j < n_keep; j += kThreads) {
+    }
+
+    // a row whose weights do not matter: all of it, or the sinks and the most recent ones
+    __device__ __forceinline__ void write_fixed() const
+    {
+        for (int j = part * kThreads + tid; j < n_keep; j += parts * kThreads) {
             const int t = all || j < a.sinks ? j : len - n_keep + j;
             kept[j] = t;
             if (j < a.cols) nw[j] = t < a.cols ? w[t] : 0.f;
         }
     }
-    for (int j = n_keep + tid; j < a.budget; j += kThreads) kept[j] = -1;
-    int64_t z = min(((int64_t)n_keep + 3) / 4 * 4, a.cols);
-    if (n_keep + tid < z) nw[n_keep + tid] = 0.f;
-    if (vec && (reinterpret_cast<uintptr_t>(a.new_weights) & 15) == 0)
-        for (z += tid * 4; z < a.cols; z += kThreads * 4) *reinterpret_cast<f32x4_t*>(nw + z) = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    else
-        for (z += tid; z < a.cols; z += kThreads) nw[z] = 0.f;
-    if (hkv == 0 && tid == 0) a.new_seqlen[b] = n_keep;
+
+    // what lies behind the kept keys
+    __device__ __forceinline__ void write_tail() const
+    {
+        const int me = part * kThreads + tid, step = parts * kThreads;
+        for (int j = n_keep + me; j < a.budget; j += step) kept[j] = -1;
+        int64_t z = min(((int64_t)n_keep + 3) / 4 * 4, a.cols);
+        if (n_keep + me < z) nw[n_keep + me] = 0.f;
+        if (vec && (reinterpret_cast<uintptr_t>(a.new_weights) & 15) == 0)
+            for (z += (int64_t)me * 4; z < a.cols; z += (int64_t)step * 4) *reinterpret_cast<f32x4_t*>(nw + z) = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        else
+            for (z += me; z < a.cols; z += step) nw[z] = 0.f;
+        if (hkv == 0 && me == 0) a.new_seqlen[b] = n_keep;
+    }
+};
+
+// one workgroup per row
+__global__ __launch_bounds__(kThreads) void evict_select_kernel(const CacheEvictArgs a)
+{
+    __shared__ SelectLds lds;
+    Select s(a, lds, blockIdx.x, 0, 1);
+    if (s.want > 0) {
+        for (int digit = 0;; ++digit) {
+            s.histogram(digit);
+            if (s.take_digit(digit)) break;
+        }
+        int sure, equal;
+        s.count(sure, equal);
+        if (s.lane == 0) {
+            lds.counts[0][s.wave] = sure;
+            lds.counts[1][s.wave] = equal;
+        }
+        __syncthreads();
+        int rank = 0, equal_left = s.left;
+        for (int v = 0; v < s.wave; ++v) {
+            const int eq = min(lds.counts[1][v], equal_left);
+            rank += lds.counts[0][v] + eq;
+            equal_left -= eq;
+        }
+        s.write(rank, equal_left);
+    } else {
+        s.write_fixed();
+    }
+    s.write_tail();
+}
+
+// kEvictParts workgroups per row, one launch per step, for few long rows: the steps hand each other their sums through the
+// workspace.  Step d = 0, 1, 2 takes the digit before (d > 0) and counts digit d of its part; step 3 takes the last digit and
+// counts what each wave keeps; step 4 writes.
+struct WideRow {
+    int hist[3][kEvictParts][kBins];
+    uint32_t state[3][4];  // after digit d: threshold, mask, left, done
+    int counts[kEvictParts * kWaves][2];
+};
+
+template <int kStep>
+__global__ __launch_bounds__(kThreads) void evict_select_wide_kernel(const CacheEvictArgs a)
+{
+    __shared__ SelectLds lds;
+    const int row = blockIdx.x / kEvictParts;
+    Select s(a, lds, row, blockIdx.x % kEvictParts, kEvictParts);
+    WideRow& ws = reinterpret_cast<WideRow*>(a.workspace)[row];
+    if (s.want == 0) {  // uniform
+        if (kStep == 4) {
+            s.write_fixed();
+            s.write_tail();
+        }
+        return;
+    }
+    bool done = false;
+    if constexpr (kStep >= 2) {
+        const uint32_t* st = ws.state[kStep == 4 ? 2 : kStep - 2];
+        s.threshold = st[0];
+        s.mask = st[1];
+        s.left = (int)st[2];
+        done = st[3] != 0;
+    }
+    if constexpr (kStep >= 1 && kStep <= 3) {
+        if (!done) {
+            for (int d = s.tid; d < kBins; d += kThreads) {
+                int sum = 0;
+#pragma unroll
+                for (int p = 0; p < kEvictParts; ++p) sum += ws.hist[kStep - 1][p][d];
+                lds.digits[d] = sum;
+            }
+            __syncthreads();
+            done = s.take_digit(kStep - 1);
+        }
+        if (s.part == 0 && s.tid == 0) {
+            uint32_t* st = ws.state[kStep - 1];
+            st[0] = s.threshold;
+            st[1] = s.mask;
+            st[2] = (uint32_t)s.left;
+            st[3] = done;
+        }
+    }
+    if constexpr (kStep <= 2) {
+        if (done) return;
+        s.histogram(kStep);
+        for (int d = s.tid; d < kBins; d += kThreads) ws.hist[kStep][s.part][d] = lds.digits[d];
+    } else if constexpr (kStep == 3) {
+        int sure, equal;
+        s.count(sure, equal);
+        if (s.lane == 0) {
+            ws.counts[s.part * kWaves + s.wave][0] = sure;
+            ws.counts[s.part * kWaves + s.wave][1] = equal;
+        }
+    } else {
+        // the counts of all waves of the row through LDS: read one by one they are a chain of round trips
+        if (s.tid < kEvictParts * kWaves * 2) lds.digits[s.tid] = ws.counts[s.tid / 2][s.tid & 1];
+        __syncthreads();
+        int rank = 0, equal_left = s.left;
+        for (int v = 0; v < s.part * kWaves + s.wave; ++v) {
+            const int eq = min(lds.digits[2 * v + 1], equal_left);
+            rank += lds.digits[2 * v] + eq;
+            equal_left -= eq;
+        }
+        s.write(rank, equal_left);
+        s.write_tail();
+    }
 }
 
 // Copies the kept rows.  A thread moves one 8- or 16-byte piece of K and of V of one KV head for kSlots consecutive slots, so
@@ -295,10 +449,25 @@ hipError_t launch_move(const CacheEvictArgs& a, hipStream_t st)
 
 }  // namespace
 
+size_t cache_evict_workspace_bytes(int64_t rows, int64_t cols, int num_cu)
+{
+    // several workgroups per row where one per row leaves most of the chip idle and the walks outweigh the extra launches
+    return rows * kEvictParts <= num_cu && cols >= kEvictWideCols ? (size_t)rows * sizeof(WideRow) : 0;
+}
+
 hipError_t launch_cache_evict(const CacheEvictArgs& a, hipStream_t st)
 {
     if ((int64_t)a.batch * a.hk > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(evict_select_kernel, dim3((unsigned)(a.batch * a.hk)), dim3(kThreads), 0, st, a);
+    const dim3 rows((unsigned)(a.batch * a.hk)), parts((unsigned)(a.batch * a.hk * kEvictParts)), threads(kThreads);
+    if (a.workspace) {
+        hipLaunchKernelGGL((evict_select_wide_kernel<0>), parts, threads, 0, st, a);
+        hipLaunchKernelGGL((evict_select_wide_kernel<1>), parts, threads, 0, st, a);
+        hipLaunchKernelGGL((evict_select_wide_kernel<2>), parts, threads, 0, st, a);
+        hipLaunchKernelGGL((evict_select_wide_kernel<3>), parts, threads, 0, st, a);
+        hipLaunchKernelGGL((evict_select_wide_kernel<4>), parts, threads, 0, st, a);
+    } else {
+        hipLaunchKernelGGL(evict_select_kernel, rows, threads, 0, st, a);
+    }
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     // rows of an odd number of 8-byte pieces (an e4m3 cache with such a head dim) are moved 8 bytes at a time
     return a.k_row % 16 == 0 && a.v_row % 16 == 0 ? launch_move<u32x4_t>(a, st) : launch_move<u32x2_t>(a, st);

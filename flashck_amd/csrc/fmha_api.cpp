@@ -1105,8 +1105,14 @@ int fck_fmha_key_weights(const void* q, const void* k, const void* lse, const vo
     return launch_status(fck::launch_key_weights(a, kernel_dim(d, d), dtype, static_cast<hipStream_t>(stream)), "key-weights launch");
 }
 
+size_t fck_fmha_cache_evict_workspace_bytes(int64_t batch, int64_t hk, int64_t cols, int64_t num_cu)
+{
+    if (batch <= 0 || hk <= 0 || cols <= 0 || batch > INT32_MAX || hk > INT32_MAX || num_cu > INT32_MAX) return 0;
+    return fck::cache_evict_workspace_bytes(batch * hk, cols, num_cu > 0 ? (int)num_cu : cu_count());
+}
+
 int fck_fmha_cache_evict(const void* k_cache, const void* v_cache, void* new_k_cache, void* new_v_cache, const void* weights,
-                         void* new_weights, const int32_t* seqlen_k, int32_t* new_seqlen_k, int32_t* kept, const int32_t* block_table,
+                         void* new_weights, void* workspace, const int32_t* seqlen_k, int32_t* new_seqlen_k, int32_t* kept, const int32_t* block_table,
                          int64_t batch_stride_block_table, int64_t page_block_size, const int32_t* new_block_table,
                          int64_t new_batch_stride_block_table, int64_t new_page_block_size, int64_t batch, int64_t hk, int64_t d, int64_t dv,
                          int64_t cols, int64_t budget, int64_t recent, int64_t sinks, int32_t dtype, void* stream)
@@ -1130,6 +1136,7 @@ int fck_fmha_cache_evict(const void* k_cache, const void* v_cache, void* new_k_c
         return fail(FCK_ERR_INVALID_ARGUMENT, "a row of new_block_table addresses %ld keys, the budget is %ld", (long)(new_batch_stride_block_table * new_page_block_size), (long)budget);
     if (block_table == new_block_table && k_cache == new_k_cache)
         return fail(FCK_ERR_INVALID_ARGUMENT, "new_block_table must name other pages than block_table: rows are not moved inside the pages that are read");
+    if (!aligned16(workspace)) return fail(FCK_ERR_INVALID_ARGUMENT, "the workspace must be 16-byte aligned");
     if (weights == new_weights) return fail(FCK_ERR_INVALID_ARGUMENT, "new_weights must not be weights");
     const int e = dtype == FCK_DTYPE_FP8 ? 1 : 2;
     fck::CacheEvictArgs a{};
@@ -1156,6 +1163,8 @@ int fck_fmha_cache_evict(const void* k_cache, const void* v_cache, void* new_k_c
     a.recent = (int32_t)recent;
     a.sinks = (int32_t)sinks;
     a.cols = cols;
+    // a workspace that the sizes have no use for is left alone
+    a.workspace = workspace && fck::cache_evict_workspace_bytes(batch * hk, cols, cu_count()) > 0 ? workspace : nullptr;
     a.k_row = (int32_t)(d * e);
     a.v_row = (int32_t)(dv * e);
     g_kernel = "evict_move_kernel";

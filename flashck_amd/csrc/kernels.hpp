@@ -190,7 +190,10 @@ struct CacheEvictArgs {
     int32_t batch, hk, budget, recent, sinks;
     int64_t cols;
     int32_t k_row, v_row;  // bytes of one head's row of K and V (multiples of 8)
+    void* workspace;       // non-null: several workgroups choose the keys of a row (cache_evict_workspace_bytes)
 };
+// bytes of workspace with which the choice of `rows` rows of `cols` weights is spread over the chip; 0: it is not worth it
+size_t cache_evict_workspace_bytes(int64_t rows, int64_t cols, int num_cu);
 hipError_t launch_cache_evict(const CacheEvictArgs& a, hipStream_t st);
 
 // arguments of the paged-cache checker: a block table (block_table != nullptr: seqlen_k, block_table_stride) or a page

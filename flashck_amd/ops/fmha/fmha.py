@@ -917,6 +917,8 @@ def shared_prefix_splits(batch, num_groups, max_group_size, q_num_heads, kv_num_
 _shared_prefix_splits = functools.lru_cache(maxsize=1024)(lambda device, *sizes: shared_prefix_splits(*sizes))
 _key_weights_row_splits = functools.lru_cache(maxsize=1024)(
     lambda device, *sizes: int(_lib.load().fck_fmha_key_weights_row_splits(*sizes, 0)))
+_evict_workspace_bytes = functools.lru_cache(maxsize=1024)(
+    lambda device, *sizes: int(_lib.load().fck_fmha_cache_evict_workspace_bytes(*sizes, 0)))
 
 
 def _check_same_device(like, **tensors):
@@ -1156,8 +1158,10 @@ def fmha_cache_evict(k_cache, v_cache, weights, seqlen_k, block_table, new_block
     if flags.flag("FC_DEBUG_KERNEL_INSTANCE"):
         validate_paged(seqlen_k=seqlen_k, block_table=block_table, num_total_pages=k_cache.shape[0], page_size=page, check=True)
         _validate_new_pages(seqlen_k, block_table, new_block_table, budget, page, nk, same_pool)
+    space = _evict_workspace_bytes(k_cache.device, B, Hk, cols)
+    space = torch.empty(space, dtype=torch.uint8, device=k_cache.device) if space else None
     with _on(k_cache):
-        _call("fck_fmha_cache_evict", _at(k_cache), _at(v_cache), _at(nk), _at(nv), _at(weights), _at(weights_new), _at(seqlen_k),
+        _call("fck_fmha_cache_evict", _at(k_cache), _at(v_cache), _at(nk), _at(nv), _at(weights), _at(weights_new), _at(space), _at(seqlen_k),
               _at(seqlen_new), _at(kept), _at(block_table), block_table.shape[1], page, _at(new_block_table), new_block_table.shape[1],
               nk.shape[1], B, Hk, D, v_cache.shape[3], cols, budget, recent, sinks, _dtype_id(k_cache), _stream())
     return seqlen_new, kept, weights_new

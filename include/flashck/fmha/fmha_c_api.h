@@ -353,17 +353,21 @@ FCK_EXPORT int fck_fmha_key_weights_row_splits(int64_t batch, int64_t q_num_head
  *                 rows go, slot j of sequence b for the j-th kept key of each head.  The pools may be the ones that are read;
  *                 the pages must then be other pages than any that block_table names (which may be shared by sequences and
  *                 are never written).
+ *   workspace     device memory of fck_fmha_cache_evict_workspace_bytes bytes (16-byte aligned; what it holds does not matter), or
+ *                 NULL: with it the choice among few long rows is spread over the chip
  * dtype is the element type of the caches.  The positions of a head's kept keys differ between heads, so masks that go by
  * position do not apply to the evicted keys.  No counterpart in the reference.
  */
 FCK_EXPORT int fck_fmha_cache_evict(const void* k_cache, const void* v_cache, void* new_k_cache, void* new_v_cache,
-                                    const void* weights, void* new_weights, const int32_t* seqlen_k,
+                                    const void* weights, void* new_weights, void* workspace, const int32_t* seqlen_k,
                                     int32_t* new_seqlen_k, int32_t* kept, const int32_t* block_table,
                                     int64_t batch_stride_block_table, int64_t page_block_size,
                                     const int32_t* new_block_table, int64_t new_batch_stride_block_table,
                                     int64_t new_page_block_size, int64_t batch, int64_t kv_num_heads, int64_t qk_head_dim,
                                     int64_t v_head_dim, int64_t cols, int64_t budget, int64_t recent, int64_t sinks,
                                     int32_t dtype, void* stream);
+/* num_cu <= 0: of the current device.  0 when one workgroup per row is as good. */
+FCK_EXPORT size_t fck_fmha_cache_evict_workspace_bytes(int64_t batch, int64_t kv_num_heads, int64_t cols, int64_t num_cu);
 
 /*
  * AppendKV: rotate knew (and q, in place) and write knew / vnew behind the seqlen_k[b] tokens each sequence

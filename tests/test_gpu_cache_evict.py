@@ -208,3 +208,14 @@ def test_on_another_stream(fmha):
     torch.cuda.synchronize()
     for p, x in zip(pools[1:], got):
         assert all(torch.equal(a, b) for a, b in zip(first, x)) and all(torch.equal(a, b) for a, b in zip(pools[0], p))
+
+
+@pytest.mark.parametrize("cols,lens", [(65536, [3000, 700]), (65546, [16390, 64]), (70000, [16100, 16100])])
+def test_wide_rows(fmha, cols, lens):
+    # rows long enough that several workgroups choose from each; distinct weights, and weights that are mostly equal
+    g = torch.Generator().manual_seed(15)
+    _run(fmha, 16, lens, 1, 8, torch.bfloat16, 64, 600, 40, 4, cols=cols, own_pool=True)
+    w = torch.randint(0, 2, (2, 1, cols), generator=g).float()
+    w[0, 0, 100:200] = math.nan
+    _run(fmha, 17, lens, 1, 8, torch.bfloat16, 64, 500, 0, 3, cols=cols, weights=w, own_pool=True)
+    _run(fmha, 18, lens, 1, 8, torch.bfloat16, 64, 44, 40, 4, cols=cols, own_pool=True)
