@@ -938,11 +938,12 @@ int fck_fmha_shared_prefix_splits(int64_t batch, int64_t num_groups, int64_t max
     for (int64_t v : {batch, num_groups, max_group_size, hq, hk, sq})
         if (v <= 0 || v > kMax) return FCK_OK;
     if (hk > hq || head_dim <= 0 || head_dim > 256 || max_prefix_len > INT32_MAX || max_own_len > INT32_MAX || num_cu > kMax) return FCK_OK;
-    // The items (a split x a KV head x a row tile) of the longest prefixes and of half the longest own keys should fill the
-    // workgroups that run at once, one round of equal ones.
+    // The items (a split x a KV head x a row tile) of the longest prefixes and of half the longest own keys make two equal ones
+    // per CU.  The small kernels leave room for three, but more partial results to merge cost more than that gives: 32 sequences
+    // on 4096 shared and up to 1024 own keys took 30 us with 16 + 4 splits (three per CU), 26 us with 11 + 3, 27 us with 10 + 2.
     const int64_t rows = max_group_size * sq * (hq / hk);
     const int d = kernel_dim(head_dim, head_dim), bm = 64 * fck::shared_prefix_blocks(d, rows);
-    const double slots = fck::shared_prefix_workgroups(d, rows, num_cu > 0 ? (int)num_cu : cu_count());
+    const double slots = 2.0 * (num_cu > 0 ? (double)num_cu : cu_count());
     const auto tiles = [&](int64_t r) { return (double)((r + bm - 1) / bm); };
     const double prefix = max_prefix_len > 0 ? (double)max_prefix_len : 0, own = max_own_len > 0 ? (double)max_own_len : 0;
     const double keys = (double)hk * (num_groups * tiles(rows) * prefix + batch * tiles(sq * (hq / hk)) * own / 2);

@@ -140,9 +140,8 @@ struct SharedPrefixArgs {
     float v_descale;
     int32_t num_cu;
 };
-// 16-row blocks per wave for groups of rows_prefix packed rows, and the workgroups that run at once with them
+// 16-row blocks per wave for groups of rows_prefix packed rows
 int shared_prefix_blocks(int d, int64_t rows_prefix);
-int shared_prefix_workgroups(int d, int64_t rows_prefix, int num_cu);
 // rows_prefix / rows_own: most packed query rows of a group / of a sequence
 hipError_t launch_shared_prefix(SharedPrefixArgs a, int d, int dtype, int64_t rows_prefix, int64_t rows_own, hipStream_t st);
 
