@@ -1139,6 +1139,8 @@ int fck_fmha_cache_evict(const void* k_cache, const void* v_cache, void* new_k_c
         return fail(FCK_ERR_INVALID_ARGUMENT, "new_block_table must name other pages than block_table: rows are not moved inside the pages that are read");
     if (!aligned16(workspace)) return fail(FCK_ERR_INVALID_ARGUMENT, "the workspace must be 16-byte aligned");
     if (weights == new_weights) return fail(FCK_ERR_INVALID_ARGUMENT, "new_weights must not be weights");
+    // the heads of a sequence read its count while one of them writes the new one
+    if (seqlen_k == new_seqlen_k) return fail(FCK_ERR_INVALID_ARGUMENT, "new_seqlen_k must not be seqlen_k");
     const int e = dtype == FCK_DTYPE_FP8 ? 1 : 2;
     fck::CacheEvictArgs a{};
     a.k = k_cache;

@@ -3,7 +3,7 @@
 // with s = mod(scale * q.k) and lse the log-sum-exp the attention over the same keys returned.  Entries at and behind a
 // sequence's key count are written as zeros, so that a key appended later starts from nothing.
 //
-// Both kernels compute S = Q . K^T with the keys as the columns of the matrix instruction: a lane owns one key per block and
+// All kernels compute S = Q . K^T with the keys as the columns of the matrix instruction: a lane owns one key per block and
 // its accumulator registers are query rows, so the sum over rows is an addition in the lane and only the few lanes that
 // hold the same key are added up at the end.  No two workgroups write the same key: there are no atomics and the order of
 // every sum is fixed.
@@ -45,7 +45,9 @@ __device__ __forceinline__ u32x4_t staged8(const char FCK_LDS* row_p, int row, i
 // Bound by reading K once.  A wave owns NT tiles of 32 keys and streams them through an LDS buffer of its own (global -> LDS
 // copies with the non-temporal hint, no workgroup barrier): a tile goes to registers as soon as it has landed and the next
 // one is requested into the same buffer, so that small buffers leave room for many waves, each with a tile in flight.  The
-// 16 MB query rows sit in registers as the A operand of v_mfma_f32_16x16x32.
+// 16 MB query rows sit in registers as the A operand of v_mfma_f32_16x16x32.  One token of 16 sequences of up to 32768 keys
+// (8 KV heads of 8 query heads, D 128, bf16): 126 us, 5.0 TB/s; the first version, through a tile shared by the workgroup
+// behind barriers, 718 us.
 template <int D, bool kKv8>
 struct StepShape {
     static constexpr int ROWB = D * (kKv8 ? 1 : 2);
@@ -421,6 +423,8 @@ __global__ __launch_bounds__(512) void key_weights_window_kernel(const KeyWeight
 //   The query tokens are cut into row_splits equal runs and a workgroup handles one run: the runs fill the chip when there
 // are few keys, and under a causal mask they make the items equal (a run is either seen whole, or crossed by the diagonal,
 // or skipped).  A run's sums go to a slice of the workspace, key_weights_sum_kernel adds the slices in order.
+//   A prompt of 8192 tokens, 32 query heads, D 128, bf16, causal: 333 us, 830 TFLOP/s of visible pairs (without a mask
+// 950 to 1036); the first version 2213 us.
 template <int D, bool kKv8>
 struct RowsShape {
     static constexpr int KW = 4, RW = 2;

@@ -15,6 +15,10 @@
 //   Prefix items come first (they are the long ones); those that stream the same keys get ids congruent modulo 8, i.e. one
 //   XCD and one L2.
 //   Every slot of every row is written (an empty one as lse = -inf), so the merge reads no lengths and no groups.
+//
+// What bounds it: a small group reads its keys (32 sequences on 4096 shared and up to 1024 own keys, 8 KV heads of 4 query
+// heads, D 128, bf16: 22 + 4 us, 3.1 TB/s), a large one multiplies (64 sequences x 8 heads on 32768 keys: 115 + 8 us,
+// 600 TFLOP/s: two products a tile with the softmax of 128 rows between them, and two waves per SIMD to overlap the two).
 #include "common.hpp"
 #include "kernels.hpp"
 

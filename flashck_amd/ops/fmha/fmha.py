@@ -1171,12 +1171,12 @@ def _validate_new_pages(seqlen_k, block_table, new_block_table, budget, page, ne
     """The pages an eviction writes: inside the pool, each used once, and none of those it reads (debug aid; synchronises)."""
     new_page = new_cache.shape[1]
     lens, old, new = seqlen_k.tolist(), block_table.tolist(), new_block_table.tolist()
-    written = [p for n, row in zip(lens, new) for p in row[:-(-min(n, budget) // new_page)]]
+    written = [p for n, row in zip(lens, new) for p in row[:-(-max(min(n, budget), 0) // new_page)]]
     if any(p < 0 or p >= new_cache.shape[0] for p in written):
         raise ValueError(f"new_block_table names a page outside the pool of {new_cache.shape[0]}")
     if len(set(written)) != len(written):
         raise ValueError("new_block_table names a page twice")
-    if same_pool and set(written) & {p for n, row in zip(lens, old) for p in row[:-(-n // page)]}:
+    if same_pool and set(written) & {p for n, row in zip(lens, old) for p in row[:-(-max(n, 0) // page)]}:
         raise ValueError("new_block_table names a page that block_table reads")
 
 

@@ -347,7 +347,7 @@ FCK_EXPORT int fck_fmha_key_weights_row_splits(int64_t batch, int64_t q_num_head
  * the first `sinks`, the last `recent` (sinks + recent <= budget) and, of the keys between, those with the largest weights
  * (ties: the lower position; a NaN counts as -inf; a position at or behind cols counts as weight 0).
  *   kept          int32 [B, Hk, budget]: the kept positions in ascending order, -1 behind the n-th
- *   new_seqlen_k  int32 [B]: n
+ *   new_seqlen_k  int32 [B]: n; must not be `seqlen_k`
  *   new_weights   fp32 [B, Hk, cols]: the weights of the kept keys, zeros behind; must not be `weights`
  *   new_k_cache, new_v_cache, new_block_table (int32 [B, new_batch_stride_block_table], >= budget keys a row): where the kept
  *                 rows go, slot j of sequence b for the j-th kept key of each head.  The pools may be the ones that are read;

@@ -1,7 +1,7 @@
 """GPU: decode attention over shared prefixes against its definition in 64 bits and against the decode without sharing.
 
 Tolerances.  Scores are products of 16-bit values summed in fp32 (relative error below 2^-20 for these lengths).  The
-kernels round the probabilities p <= 1 to the 16-bit type before the second product, off by at most half a step, u = 2^-8
+kernels round the probabilities (a row's common factor apart) to the 16-bit type before the second product, off by at most half a step, u = 2^-8
 (bf16) or 2^-11 (fp16) relative, and the result once more.  So |o - o_ref| <= u * sum_j p_j |v_j| + u * |o| <= 2 u max|v|;
 the values are normal, max|v| < 6, and 2^-20 more covers the fp32 parts.  The log-sum-exp is fp32 throughout: 2e-5
 absolute for |lse| < 16 (a dozen fp32 steps, the hardware's exp2 and log2 being off by about one each)."""
@@ -60,6 +60,32 @@ def test_one_group(fmha, dtype, hq, hk, d, page):
     for nsp, nso in ((0, 0), (1, 1), (3, 2)):
         o, lse = _run(fmha, c, num_prefix_splits=nsp, num_splits=nso)
         _check(o, lse, *ref, dtype, f"splits {nsp} {nso}")
+
+
+@pytest.mark.parametrize("splits", [(64, 64), (64, 1), (1, 64)])
+def test_most_splits(fmha, splits):
+    c = _case(23, [2, 3], [700, 0], [0, 513, 64], 8, 2, 64, torch.bfloat16, 64)
+    o, lse = _run(fmha, c, num_prefix_splits=splits[0], num_splits=splits[1])
+    _check(o, lse, *lc.decode(c["q"], c["kc"], c["vc"], c["lens"], c["table"], 0.125), torch.bfloat16, f"{splits}")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("step", [0.75, 4.0, 16.0])
+def test_scores_that_grow_along_the_keys(fmha, dtype, step):
+    # the largest score of every tile outgrows that of the tile before by less and by more than any reference of the
+    # exponents may lag behind; rows of the group grow, fall and stay, in one wave.  q = (c, 0, ..), k = (step * tile, ..)
+    c = _case(24, [16], [64 * 9], [5, 64], 1, 1, 64, dtype, 64)
+    c["q"].zero_()
+    c["q"][:, 0, 0, 0] = torch.tensor([1.0, -1.0, 0.0, 0.5] * 4)
+    for b, n in enumerate(c["lens"]):
+        for t in range(n):
+            c["kc"][int(c["table"][b, t // 64]), t % 64, 0, 0] = step * (t // 64)
+    ref = lc.decode(c["q"], c["kc"], c["vc"], c["lens"], c["table"], 1.0)
+    for splits in ((1, 1), (3, 1)):
+        o, lse = _run(fmha, c, scale=1.0, num_prefix_splits=splits[0], num_splits=splits[1])
+        assert (o.double() - ref[0]).abs().max() <= (2 * U[dtype] + 2.0 ** -20) * 6.0
+        # |score| reaches 144: an fp32 step there is 2^-16
+        assert (lse.double() - ref[1]).abs().max() <= 1e-4
 
 
 @pytest.mark.parametrize("rows", [1, 15, 16, 17, 33, 70])

@@ -145,6 +145,7 @@ def test_debug_flag_checks_the_pages_an_eviction_writes(ops):
             F._validate_new_pages(_i32(20, 17), old, _i32(*new).view(2, 1), 16, 16, k, True)
     F._validate_new_pages(_i32(20, 17), old, _i32(4, 3).view(2, 1), 16, 16, k, False)   # a pool of its own
     F._validate_new_pages(_i32(20, 0), old, _i32(4, 99).view(2, 1), 16, 16, k, True)    # an empty sequence writes no page
+    F._validate_new_pages(_i32(20, -40), old, _i32(4, 99).view(2, 1), 16, 16, k, True)  # nor does one of negative length
 
 
 def test_the_step_and_the_module_reach_the_operators(ops, monkeypatch):
@@ -226,7 +227,7 @@ def test_abi_key_weights(kw, rc):
 
 
 def _abi_evict(**kw):
-    a = dict(k=P, v=P, nk=P, nv=P, w=P, nw=ctypes.c_void_p(1 << 21), ws=None, sk=P, nsk=P, kept=P, bt=P, stride=2, page=16, nbt=ctypes.c_void_p(1 << 21),
+    a = dict(k=P, v=P, nk=P, nv=P, w=P, nw=ctypes.c_void_p(1 << 21), ws=None, sk=P, nsk=ctypes.c_void_p(1 << 22), kept=P, bt=P, stride=2, page=16, nbt=ctypes.c_void_p(1 << 21),
              nstride=1, npage=16, batch=2, hk=2, d=64, dv=64, cols=32, budget=16, recent=0, sinks=0, dtype=4, stream=None)
     a.update(kw)
     return _lib.load().fck_fmha_cache_evict(*a.values())
@@ -235,7 +236,7 @@ def _abi_evict(**kw):
 @pytest.mark.parametrize("kw,rc", [
     (dict(k=None), -1), (dict(kept=None), -1), (dict(nk=ctypes.c_void_p(8)), -1), (dict(budget=0), -1), (dict(budget=17), -1), (dict(recent=17), -1),
     (dict(recent=9, sinks=8), -1), (dict(sinks=-1), -1), (dict(dtype=0), -2), (dict(d=10), -2), (dict(dv=512), -2), (dict(nbt=P), -1), (dict(nw=P), -1),
-    (dict(ws=ctypes.c_void_p(8)), -1),
+    (dict(ws=ctypes.c_void_p(8)), -1), (dict(nsk=P), -1),
     (dict(cols=0), -1), (dict(npage=0), -1), (dict(batch=1 << 30, hk=4), -1),
 ])
 def test_abi_evict(kw, rc):
