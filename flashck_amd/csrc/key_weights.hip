@@ -131,7 +131,8 @@ __global__ __launch_bounds__(256) void key_weights_step_kernel(const KeyWeightsA
         for (int v = 0; v < 4; ++v) {
             const int r = mb * 16 + kg * 4 + v;
             const int i = r < R ? r / g : 0, h = hkv * g + (r < R ? r % g : 0);
-            // a row that does not exist, or that saw no key, gives exp2(-inf) = 0
+            // a row that does not exist, or that saw no key, adds nothing: lse2 = +inf gives exp2(-inf) = 0 for a finite score, and the
+            // terms of scores that are not (a key with an infinite element) are left out by selection
             lse2[mb][v] = INFINITY;
             if (r < R) {
                 const float l = a.lse[((int64_t)(a.seqstart_q ? 0 : b) * a.hq + h) * a.lse_sq + (a.seqstart_q ? tok0 : 0) + i];
@@ -198,7 +199,7 @@ __global__ __launch_bounds__(256) void key_weights_step_kernel(const KeyWeightsA
                         e = fast_exp2(amod[mb][v].score(s[nb][mb][v], key) - lse2[mb][v]);
                     else
                         e = fast_exp2(__builtin_fmaf(s[nb][mb][v], a.scale_log2, -lse2[mb][v]));
-                    x += all || (key >= lo[mb][v] && key < hi[mb][v]) ? e : 0.f;
+                    x += (all || (key >= lo[mb][v] && key < hi[mb][v])) && lse2[mb][v] != INFINITY ? e : 0.f;
                 }
             sum[nb] = quad16_sum(x);
         }
@@ -230,11 +231,11 @@ struct WindowShape {
     static constexpr int NT = 4;  // key tiles per wave
     static constexpr int KEYS = 8 * NT * 32;
     static constexpr int MAX_ROWS = 65536 / QB;
-    static constexpr size_t lds(int rows32) { return 8 * TILEB + 8 * NT * 32 * 4 + (size_t)rows32 * (QB + 8); }
+    static constexpr size_t lds(int rows32) { return 8 * TILEB + 8 * NT * 32 * 4 + (size_t)rows32 * (QB + 8) + rows32 / 32 * 4; }
 };
 
-// Tokens [first, end) see key `key`: the mask [mask_lo, mask_hi) of a token, solved for the token.  A row that does not exist
-// has token INT32_MAX, which no range holds.
+// Tokens [first, end) see key `key`: the mask [mask_lo, mask_hi) of a token, solved for the token.  A row that does not exist,
+// or whose lse is -inf, has token INT32_MAX, which no range holds: it adds nothing whatever its scores are.
 struct Seen {
     int32_t first, end;
 };
@@ -313,6 +314,7 @@ __global__ __launch_bounds__(512) void key_weights_window_kernel(const KeyWeight
     char FCK_LDS* const qs = (char FCK_LDS*)smem + 8 * S::TILEB + 8 * S::NT * 32 * 4;
     float FCK_LDS* const row_lse = (float FCK_LDS*)(qs + rows32 * S::QB);
     int FCK_LDS* const row_tok = (int FCK_LDS*)(row_lse + rows32);
+    int FCK_LDS* const block_full = row_tok + rows32;  // every row of the 32-row block adds something
 
     const KvSeq ks = kv_seq(a.kv, b);
     const int sk = __builtin_amdgcn_readfirstlane(max(ks.len, 0));
@@ -369,12 +371,18 @@ __global__ __launch_bounds__(512) void key_weights_window_kernel(const KeyWeight
             v = ldg16((const char*)a.q + ((int64_t)(tok0 + row / g) * a.hq + hkv * g + row % g) * q_bytes + chunk * 16);
         *(u32x4_t FCK_LDS*)(qs + row * S::QB + ((chunk ^ chunk_swizzle<S::QCH>(row)) << 4)) = v;
     }
-    for (int row = tid; row < rows32; row += 512) {
+    for (int row0 = wave * 64; row0 < rows32; row0 += 512) {  // whole waves: two blocks
+        const int row = row0 + lane;
         float l = -INFINITY;
         if (row < R) l = a.lse[((int64_t)(a.seqstart_q ? 0 : b) * a.hq + hkv * g + row % g) * a.lse_sq + (a.seqstart_q ? tok0 : 0) + row / g];
-        // a row that does not exist, or that saw no key, gives exp2(-inf) = 0
-        row_lse[row] = l == -INFINITY ? INFINITY : l * kLog2e;
-        row_tok[row] = row < R ? row / g : INT32_MAX;
+        // a row that does not exist, or that saw no key, adds nothing
+        const bool none = l == -INFINITY;
+        const uint64_t nones = __builtin_amdgcn_ballot_w64(none);
+        if (row < rows32) {
+            row_lse[row] = none ? INFINITY : l * kLog2e;
+            row_tok[row] = none ? INT32_MAX : row / g;
+            if (l32 == 0) block_full[row / 32] = (uint32_t)(nones >> (half * 32)) == 0;
+        }
     }
     __syncthreads();
 
@@ -397,7 +405,7 @@ __global__ __launch_bounds__(512) void key_weights_window_kernel(const KeyWeight
 #pragma unroll
             for (int t = 0; t < S::KT; ++t)
                 s[0] = T::mfma32(as_vec8<vec8>(staged8<T, false, S::QCH>(qs + (rs + l32) * S::QB, rs + l32, t * 2 + half)), as_vec8<vec8>(kf[t]), s[0]);
-            const bool all = mask_lo(mk, i_last) <= kb && mask_hi(mk, i_first, sk) >= min(kb + 32, sk);  // rows that do not exist add 0
+            const bool all = __builtin_amdgcn_readfirstlane(block_full[rs / 32]) != 0 && mask_lo(mk, i_last) <= kb && mask_hi(mk, i_first, sk) >= min(kb + 32, sk);
             add_block<T, kMod, 1>(a, mk, acc, s, row_lse + rs + half * 4, row_tok + rs + half * 4, all, rs + half * 4, kb + l32, b, hkv * g, g, sq, sk);
         }
         return pair32_sum(acc[0]);
@@ -437,7 +445,7 @@ struct RowsShape {
     static constexpr int LDQ = STAGEB / 8192, LDK = KEYS * KB / 8192;  // copies per wave
     static constexpr int RPL = 1024 / QB;                              // query rows per copy
     static constexpr int KT = D / 16;
-    static constexpr size_t lds = 2 * STAGEB + 2 * ROWS * 12 + RW * KEYS * 4;
+    static constexpr size_t lds = 2 * STAGEB + 2 * ROWS * 12 + RW * KEYS * 4 + 2 * (ROWS / 64) * 4;
     static_assert(KEYS * KB <= 2 * STAGEB && KEYS * KB % 8192 == 0 && STAGEB % 8192 == 0, "the key tile passes through the stage buffers");
     static_assert(ROWS <= 512, "one thread per staged row");
 };
@@ -448,11 +456,12 @@ __global__ __launch_bounds__(512) void key_weights_rows_kernel(const KeyWeightsA
     typedef RowsShape<D, kKv8> S;
     typedef typename T::vec8 vec8;
     FCK_DYNAMIC_LDS(smem);
-    char FCK_LDS* const lds = (char FCK_LDS*)smem;  // two stages (or the key tile) | of their rows: lse, token, -lse / scale | sums
+    char FCK_LDS* const lds = (char FCK_LDS*)smem;  // two stages (or the key tile) | of their rows: lse, token, -lse / scale | sums | pairs of row blocks
     float FCK_LDS* const row_lse = (float FCK_LDS*)(lds + 2 * S::STAGEB);
     int FCK_LDS* const row_tok = (int FCK_LDS*)(row_lse + 2 * S::ROWS);
     float FCK_LDS* const row_init = (float FCK_LDS*)(row_tok + 2 * S::ROWS);
     float FCK_LDS* const sums = row_init + 2 * S::ROWS;
+    int FCK_LDS* const pair_none = (int FCK_LDS*)(sums + S::RW * S::KEYS);  // some of the 64 rows adds nothing
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -579,11 +588,14 @@ __global__ __launch_bounds__(512) void key_weights_rows_kernel(const KeyWeightsA
         };
         auto publish = [&](int st) __attribute__((always_inline)) {
             if (tid < S::ROWS) {
-                // a row that saw no key gives exp2(-inf) = 0
-                const float l = lse_next == -INFINITY ? INFINITY : lse_next * kLog2e;
+                // a row that saw no key adds nothing: the pair of row blocks it lies in takes the path that selects by token
+                const bool none = lse_next == -INFINITY;
+                const float l = none ? INFINITY : lse_next * kLog2e;
                 row_lse[(st & 1) * S::ROWS + tid] = l;
                 row_init[(st & 1) * S::ROWS + tid] = -l / a.scale_log2;
-                row_tok[(st & 1) * S::ROWS + tid] = tok_next;
+                row_tok[(st & 1) * S::ROWS + tid] = none ? INT32_MAX : tok_next;
+                const uint64_t nones = __builtin_amdgcn_ballot_w64(none);
+                if (lane == 0) pair_none[(st & 1) * (S::ROWS / 64) + wave] = nones != 0;
             }
         };
         // The block pipeline of the tiles every row sees: while the matrix instructions of a block run, the exponentials of
@@ -651,6 +663,10 @@ __global__ __launch_bounds__(512) void key_weights_rows_kernel(const KeyWeightsA
             publish(st);
             __syncthreads();
             if (st + 1 < stages) request(st + 1);
+            uint32_t none = 0;  // bit p: pair p of this wave's rows
+#pragma unroll
+            for (int p = 0; p < S::SUB / 2; ++p) none |= (uint32_t)pair_none[(st & 1) * (S::ROWS / 64) + rw * (S::SUB / 2) + p] << p;
+            none = __builtin_amdgcn_readfirstlane(none);
 #pragma unroll 1
             for (int pair = 0; pair < S::SUB / 2; ++pair) {
                 const int rl = (rw * S::SUB + pair * 2) * 32;  // this wave's rows in the stage, 64 at a time
@@ -660,7 +676,7 @@ __global__ __launch_bounds__(512) void key_weights_rows_kernel(const KeyWeightsA
                 const float FCK_LDS* lp = row_lse + (st & 1) * S::ROWS + rl + half * 4;
                 const float FCK_LDS* ip = row_init + (st & 1) * S::ROWS + rl + half * 4;
                 const int FCK_LDS* tp = row_tok + (st & 1) * S::ROWS + rl + half * 4;
-                if (!kMod && rs >= all_lo && rs + 64 <= all_hi) {
+                if (!kMod && (none >> pair & 1) == 0 && rs >= all_lo && rs + 64 <= all_hi) {
                     if (pending)
                         block(0, q0, ip, std::true_type{}, std::true_type{});
                     else

@@ -1,0 +1,45 @@
+"""The GPU tests of the operators' corners (test_gpu_operator_edges) on the wave64 emulator (see test_emu_kernels.py), all of
+them: the unchanged kernel sources, CPU tensors against guard pages."""
+import importlib
+
+import pytest
+import torch
+
+import test_emu_kernels as emu
+
+GPU_MODULES = ["test_gpu_operator_edges"]
+NEEDS_DEVICE = set()
+
+_mods = [importlib.import_module(m) for m in GPU_MODULES]
+for _m in _mods:
+    for _name in dir(_m):
+        _fn = getattr(_m, _name)
+        if _name.startswith("test_") and callable(_fn) and _name not in NEEDS_DEVICE:
+            globals()[f"test_emu_{_m.__name__[9:]}__{_name[5:]}"] = _fn
+del _fn
+
+
+@pytest.fixture(scope="module")
+def fmha():
+    import ctypes
+    import build_emu
+    import helpers
+    from flashck_amd import _lib
+    from flashck_amd.ops import fmha as ops
+    from flashck_amd.ops.fmha import fmha as F
+    lib = ctypes.CDLL(build_emu.build())
+    for name, (res, args) in _lib.SIGNATURES.items():
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = res, args
+    saved = (_lib._lib, F._REQUIRE_GPU_TENSORS, F._stream, torch.cuda.synchronize, helpers.DEVICE, [(m, m.dev) for m in _mods])
+    _lib._lib, F._REQUIRE_GPU_TENSORS, F._stream = lib, False, (lambda: None)
+    torch.cuda.synchronize = lambda *a, **k: None
+    helpers.DEVICE = "cpu"
+    for m in _mods:
+        m.dev = emu._cpu
+    try:
+        yield ops
+    finally:
+        _lib._lib, F._REQUIRE_GPU_TENSORS, F._stream, torch.cuda.synchronize, helpers.DEVICE, devs = saved
+        for m, d in devs:
+            m.dev = d

@@ -1,0 +1,73 @@
+"""GPU: the corners of the operators on long shared caches, against their definitions in 64 bits: keys whose scores are not
+finite, rows that add nothing, caches with more keys than the weights have columns.
+
+Tolerances are those of test_gpu_key_weights (REL) and test_gpu_shared_prefix (U), derived there."""
+import math
+
+import pytest
+import torch
+
+import longcontext as lc
+from helpers import dev
+
+pytestmark = pytest.mark.gpu
+REL = 2.5e-5
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def _i32(x):
+    return dev(torch.tensor(x, dtype=torch.int32))
+
+
+def _weights_case(seed, lens, sq, hq, hk, d, dtype, page, minus_inf=(), **kw):
+    """Inputs of fmha_key_weights; the keys `minus_inf` of every sequence score -inf for every row."""
+    g = torch.Generator().manual_seed(seed)
+    kc, _, table = lc.pages(g, lens, page, hk, d, d, dtype)
+    q = lc.randn(g, len(lens), sq, hq, d, dtype=dtype)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    for b, n in enumerate(lens):
+        for t in minus_inf:
+            if t < n:
+                kc[table[b, t // page], t % page, :, 0] = -math.inf
+    keys = [lc.rows(kc, table[b], n, page) for b, n in enumerate(lens)]
+    _, lse = lc.decode(q, kc, torch.zeros_like(kc), lens, table, d ** -0.5, **kw)
+    return dict(q=q, kc=kc, table=table, lens=lens, keys=keys, lse=lse.float())
+
+
+def _weights(fmha, c, **kw):
+    return fmha.fmha_key_weights(dev(c["q"]), dev(c["kc"]), dev(c["lse"]), _i32(c["lens"]), dev(c["table"]), **kw).cpu()
+
+
+def _close(got, want, what=""):
+    assert got.shape == want.shape and torch.isfinite(got).all(), f"{what}: not finite"
+    err = ((got.double() - want).abs() - REL * want).max().item()
+    assert err <= 1e-9, f"{what}: off by {err:.3e} beyond the relative bound"
+
+
+# (sq, hq, hk, d): one and two 16-row blocks in registers, partly and wholly filled; rows in LDS; rows that are streamed
+ROWS = [(1, 4, 1, 64), (1, 16, 1, 128), (2, 8, 2, 256), (5, 4, 1, 128), (33, 1, 1, 64), (33, 4, 2, 128), (64, 1, 1, 128),
+        (40, 1, 1, 256), (290, 2, 1, 128), (290, 2, 1, 64)]
+
+
+@pytest.mark.parametrize("mask", [dict(), dict(mask_type=2, window=(-1, 0))])
+@pytest.mark.parametrize("sq,hq,hk,d", ROWS)
+def test_a_visible_key_of_score_minus_infinity_receives_nothing(fmha, sq, hq, hk, d, mask):
+    lens = [sq + 70, 63] if sq < 63 else [sq + 70]
+    c = _weights_case(1, lens, sq, hq, hk, d, torch.float16, 64, minus_inf=(5, 40, 62), **mask)
+    want = lc.key_weights(c["q"], c["keys"], c["lse"], max(lens), d ** -0.5, **mask)
+    assert not want[:, :, 5].any() and not want[:, :, 40].any() and want[:, :, 6].any()
+    _close(_weights(fmha, c, max_seqlen_k=max(lens), **mask), want)
+
+
+@pytest.mark.parametrize("mask", [dict(), dict(mask_type=2, window=(-1, 0))])
+@pytest.mark.parametrize("sq,hq,hk,d", ROWS)
+def test_rows_whose_lse_is_minus_infinity_add_nothing_whatever_they_hold(fmha, sq, hq, hk, d, mask):
+    # padded rows: queries and scores of theirs may be anything
+    c = _weights_case(2, [sq + 70], sq, hq, hk, d, torch.bfloat16, 64, **mask)
+    g = torch.Generator().manual_seed(3)
+    none = torch.rand(1, hq, sq, generator=g) < 0.1
+    none[0, hq - 1, sq - 1] = True
+    c["lse"][none] = -math.inf
+    want = lc.key_weights(c["q"], c["keys"], c["lse"], sq + 70, d ** -0.5, **mask)
+    c["q"][none.permute(0, 2, 1)] = math.nan
+    _close(_weights(fmha, c, max_seqlen_k=sq + 70, **mask), want)
