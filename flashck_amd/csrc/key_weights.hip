@@ -80,7 +80,9 @@ __global__ __launch_bounds__(256) void key_weights_step_kernel(const KeyWeightsA
     const KvSeq ks = kv_seq(a.kv, b);
     const int sk = __builtin_amdgcn_readfirstlane(max(ks.len, 0));
     const int64_t row_out = ((int64_t)b * a.hk + hkv) * a.cols;
-    const int n = key0 < sk ? (int)min((int64_t)NT, (sk - key0 + 31) / 32) : 0;  // tiles that hold keys
+    // tiles that hold keys with a column: what is requested is waited for before the wave ends
+    const int64_t key1 = min((int64_t)sk, a.cols);
+    const int n = key0 < key1 ? (int)min((int64_t)NT, (key1 - key0 + 31) / 32) : 0;
 
     const bool uniform = ks.table == nullptr || a.kv.page_size % 32 == 0;  // a tile never straddles a page
     const char* const kp = (const char*)a.k;
@@ -322,7 +324,8 @@ __global__ __launch_bounds__(512) void key_weights_window_kernel(const KeyWeight
     const int sq = __builtin_amdgcn_readfirstlane(a.seqstart_q ? a.seqstart_q[b + 1] - tok0 : a.sq);
     const MaskYX mk = make_mask(a.mask_type, a.window_left, a.window_right, sq, sk);
     const int64_t row_out = ((int64_t)b * a.hk + hkv) * a.cols;
-    const int n = key0 < sk ? (int)min((int64_t)S::NT, (sk - key0 + 31) / 32) : 0;
+    const int64_t key1 = min((int64_t)sk, a.cols);  // tiles that hold keys with a column, as above
+    const int n = key0 < key1 ? (int)min((int64_t)S::NT, (key1 - key0 + 31) / 32) : 0;
     const int R = min(sq * g, rows32);
     const int q_bytes = a.d * 2, k_bytes = a.d * (kKv8 ? 1 : 2);
 

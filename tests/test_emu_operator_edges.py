@@ -1,6 +1,8 @@
-"""The GPU tests of the operators' corners (test_gpu_operator_edges) on the wave64 emulator (see test_emu_kernels.py), all of
-them: the unchanged kernel sources, CPU tensors against guard pages."""
+"""The GPU tests of the operators' corners (test_gpu_operator_edges) on the wave64 emulator (see test_emu_kernels.py): the
+unchanged kernel sources, CPU tensors against guard pages.  By default without the cases of SLOW, with FCK_EMU_FULL=1 all."""
 import importlib
+import os
+import re
 
 import pytest
 import torch
@@ -9,6 +11,8 @@ import test_emu_kernels as emu
 
 GPU_MODULES = ["test_gpu_operator_edges"]
 NEEDS_DEVICE = set()
+# seconds each; the other cases reach the same code, or a case that stays in does
+SLOW = re.compile(r"mask1|fewer_columns_than_keys\[64-.-.*-(1|40|64|130|199)\]|fewer_columns_than_keys\[64-5|infinity_receives_nothing\[290-2-1-64")
 
 _mods = [importlib.import_module(m) for m in GPU_MODULES]
 for _m in _mods:
@@ -17,6 +21,12 @@ for _m in _mods:
         if _name.startswith("test_") and callable(_fn) and _name not in NEEDS_DEVICE:
             globals()[f"test_emu_{_m.__name__[9:]}__{_name[5:]}"] = _fn
 del _fn
+
+
+@pytest.fixture(autouse=True)
+def _quick_set(request):
+    if os.environ.get("FCK_EMU_FULL") != "1" and SLOW.search(request.node.name):
+        pytest.skip("not in the emulator's quick set; FCK_EMU_FULL=1 runs it")
 
 
 @pytest.fixture(scope="module")

@@ -71,3 +71,22 @@ def test_rows_whose_lse_is_minus_infinity_add_nothing_whatever_they_hold(fmha, s
     want = lc.key_weights(c["q"], c["keys"], c["lse"], sq + 70, d ** -0.5, **mask)
     c["q"][none.permute(0, 2, 1)] = math.nan
     _close(_weights(fmha, c, max_seqlen_k=sq + 70, **mask), want)
+
+
+@pytest.mark.parametrize("cols", [1, 40, 64, 65, 130, 199])
+@pytest.mark.parametrize("batch,sq,hq,hk,d", [(64, 1, 8, 8, 64), (64, 5, 32, 8, 64), (1, 33, 4, 2, 128), (2, 33, 1, 1, 64), (1, 290, 2, 1, 64)])
+def test_fewer_columns_than_keys(fmha, batch, sq, hq, hk, d, cols):
+    # the first two: enough sequences that a wave walks eight tiles.  No tile without a column may be asked for.
+    few = min(4, batch)   # sequences 4.. are copies of the first four
+    lens = [200 - 7 * b for b in range(few)]
+    g = torch.Generator().manual_seed(4)
+    kc, _, table = lc.pages(g, lens, 64, hk, d, d, torch.bfloat16)
+    q, lse = lc.randn(g, few, sq, hq, d, dtype=torch.bfloat16), torch.full((few, hq, sq), 5.0)
+    before = torch.rand(few, hk, cols, generator=g)
+    want = lc.key_weights(q, [lc.rows(kc, table[b], n, 64) for b, n in enumerate(lens)], lse, cols, d ** -0.5, before=before)
+    copies = lambda x: x.repeat(-(-batch // few), *[1] * (x.dim() - 1))[:batch].contiguous()
+    args = (dev(copies(q)), dev(kc), dev(copies(lse)), dev(copies(torch.tensor(lens, dtype=torch.int32))), dev(copies(table)))
+    w = dev(copies(before))
+    out = fmha.fmha_key_weights(*args, weights=w)
+    _close(out.cpu(), copies(want))
+    assert fmha.fmha_key_weights(*args, weights=w, out=w) is w and torch.equal(w.cpu(), out.cpu())
