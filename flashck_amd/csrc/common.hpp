@@ -202,14 +202,15 @@ __device__ __forceinline__ f32x4_t combine_splits(const float* lse_acc, const fl
 #pragma unroll
         for (int j = 1; j < kCombineBatch; ++j) mb = fmaxf(mb, l[j]);
         const float m_new = fmaxf(m_run, mb);
-        if (m_new == -INFINITY) continue;
-        const float keep = __expf(m_run - m_new);  // 0 for the first non-empty batch
+        // no finite reference yet: every split so far is empty (weight 0) or NaN (the row is NaN, and stays it)
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float keep = __expf(m_run - m_use);  // 0 for the first non-empty batch
         sum *= keep;
 #pragma unroll
         for (int k = 0; k < 4; ++k) acc[k] *= keep;
 #pragma unroll
         for (int j = 0; j < kCombineBatch; ++j) {
-            const float wgt = __expf(l[j] - m_new);
+            const float wgt = __expf(l[j] - m_use);
             sum += wgt;
             if (wgt != 0.f) {  // an empty split's partial row may hold anything
 #pragma unroll

@@ -90,3 +90,34 @@ def test_fewer_columns_than_keys(fmha, batch, sq, hq, hk, d, cols):
     out = fmha.fmha_key_weights(*args, weights=w)
     _close(out.cpu(), copies(want))
     assert fmha.fmha_key_weights(*args, weights=w, out=w) is w and torch.equal(w.cpu(), out.cpu())
+
+
+def _shared_case(seed, lens, prefix, sq, hq, hk, d, dtype, page):
+    """One group: the sequences share the first `prefix` tokens."""
+    g = torch.Generator().manual_seed(seed)
+    kc, vc, table = lc.pages(g, lens, page, hk, d, d, dtype)
+    lc.share(kc, vc, table, [0, len(lens)], [prefix], page)
+    return dict(q=lc.randn(g, len(lens), sq, hq, d, dtype=dtype), kc=kc, vc=vc, table=table, lens=lens)
+
+
+@pytest.mark.parametrize("splits", [1, 2, 20])
+def test_a_row_of_nan_is_nan_after_the_merge(fmha, splits):
+    # a NaN query, and a query that meets an infinite key: the row's splits are all NaN, or some are; other rows do not notice
+    lens = [700, 650, 3]
+    c = _shared_case(5, lens, 3, 1, 4, 2, 64, torch.float16, 64)
+    c["q"][0, 0, 1] = math.nan
+    c["q"][:, 0, 2:, 0] = c["q"][:, 0, 2:, 0].abs() + 0.5
+    c["kc"][c["table"][:, 0].long(), 2, 1, 0] = math.inf   # a key of the prefix
+    bad = torch.zeros(3, 4, dtype=torch.bool)
+    bad[0, 1] = True
+    bad[:, 2:] = True
+    ref, ref_lse = lc.decode(torch.nan_to_num(c["q"]), torch.nan_to_num(c["kc"], posinf=0.0, nan=0.0), c["vc"], lens, c["table"], 0.125)
+    args = (dev(c["q"]), dev(c["kc"]), dev(c["vc"]), _i32(lens), dev(c["table"]))
+    lse, lse2 = dev(torch.zeros(3, 4, 1)), dev(torch.zeros(3, 4, 1))
+    o = fmha.fmha_decode_paged(*args, num_splits=splits, lse=lse)
+    o2 = fmha.fmha_decode_shared_prefix(*args, _i32([3]), num_prefix_splits=1, num_splits=splits, lse=lse2)
+    for got, got_lse in ((o, lse), (o2, lse2)):
+        got, got_lse = got.cpu()[:, 0], got_lse.cpu()[..., 0]
+        assert torch.isnan(got[bad]).all() and torch.isnan(got_lse[bad]).all()
+        assert (got.double() - ref[:, 0])[~bad].abs().max() <= (2 * U[torch.float16] + 2.0 ** -20) * 6.0
+        assert (got_lse.double() - ref_lse[..., 0])[~bad].abs().max() <= 2e-5
