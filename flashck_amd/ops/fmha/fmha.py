@@ -239,6 +239,22 @@ def _debug_validate(**kw):
         validate_paged(check=True, **kw)
 
 
+def _read_entries(block_table, seqlen_k, prefix_lens, cu_groups, max_group_size, page, append=False):
+    """The table a step over shared prefixes uses, for the debug flag's check (synchronises): whole pages of a prefix come from the
+    row of the group's first sequence, whatever the other rows hold there.  append: seqlen_k are the lengths before an append, which
+    goes to the pages of a sequence's own row."""
+    table, lens, B = block_table.clone(), seqlen_k.tolist(), seqlen_k.numel()
+    cu = [0, B] if cu_groups is None else [min(max(x, 0), B) for x in cu_groups.tolist()]
+    for first, end, prefix in zip(cu, cu[1:], prefix_lens.tolist()):
+        end = min(end, first + max_group_size) if max_group_size > 0 else end
+        if first < end:
+            whole = min(max(prefix, 0), max(lens[first], 0), table.shape[1] * page) // page
+            for b in range(first + 1, end):
+                n = min(whole, max(lens[b], 0) // page) if append else whole
+                table[b, :n] = block_table[first, :n]
+    return table
+
+
 def fused_reset() -> None:
     """Zero the arrival tickets of fmha_fwd_splitkv_fused on the current device and forget which stream owns which slice
     of the library's array (after a fused launch that did not run to completion, or to serve other streams; only while
@@ -501,12 +517,14 @@ def fmha_fwd_splitkv_combine(lse_acc, o_acc, dtype, cu_seqlens_q=None, max_seqle
 
 def fmha_fwd_appendkv(q, k_cache, v_cache, knew, vnew, seqlen_k, *, cu_seqlens_knew=None, max_seqlen_knew: int = 0,
                       rotary_cos=None, rotary_sin=None, rope_mode: int = ROPE_NONE, has_mask: bool = True,
-                      block_table=None, cache_batch_idx=None, k_descale: float = 1.0, v_descale: float = 1.0) -> None:
+                      block_table=None, cache_batch_idx=None, k_descale: float = 1.0, v_descale: float = 1.0,
+                      _read_table=None) -> None:
     """Rotate knew (and q, in place) and append knew/vnew to the cache behind seqlen_k[b] tokens; in place.
 
     knew/vnew/q are packed [total_new, H, D] with cu_seqlens_knew, or [B, n, H, D] with n new tokens everywhere.
     seqlen_k is NOT advanced: the caller adds the new counts, as with the ck_tile kernel.
     torch.float8_e4m3fn caches are written quantised with the static scales: cache = fp8(x / descale), saturating.
+    _read_table: what the debug flag's check walks in place of block_table (see _read_entries).
     """
     packed = cu_seqlens_knew is not None
     _check_tensor("knew", knew, ndim=3 if packed else 4)
@@ -554,8 +572,8 @@ def fmha_fwd_appendkv(q, k_cache, v_cache, knew, vnew, seqlen_k, *, cu_seqlens_k
         stride, page, rows = block_table.shape[1], k_cache.shape[1], 0
         if flags.flag("FC_DEBUG_KERNEL_INSTANCE"):  # the table must hold the sequences WITH their new tokens
             grown = seqlen_k + ((cu_seqlens_knew[1:] - cu_seqlens_knew[:-1]) if packed else n)
-            validate_paged(seqlen_k=grown.to(torch.int32), block_table=block_table, num_total_pages=k_cache.shape[0],
-                           page_size=page, check=True)
+            validate_paged(seqlen_k=grown.to(torch.int32), block_table=block_table if _read_table is None else _read_table,
+                           num_total_pages=k_cache.shape[0], page_size=page, check=True)
     else:
         stride, page, rows = 0, 0, k_cache.shape[1]
     args = (_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(knew), _ptr(vnew), _ptr(seqlen_k), _ptr(cu_seqlens_knew), n,
@@ -863,9 +881,12 @@ def fmha_decode_step(q, knew, vnew, k_cache, v_cache, seqlen_k, block_table, *, 
         if q.dim() != 4:
             raise ValueError(f"q must be [B, n, Hq, D] without cu_seqlens_knew, got shape {tuple(q.shape)}")
         n = q.shape[1]
+    read_table = None
+    if prefix_lens is not None and flags.flag("FC_DEBUG_KERNEL_INSTANCE"):
+        read_table = _read_entries(block_table, seqlen_k, prefix_lens, cu_groups, max_group_size, page, append=True)
     fmha_fwd_appendkv(q, k_cache, v_cache, knew, vnew, seqlen_k, cu_seqlens_knew=cu_seqlens_knew, max_seqlen_knew=n,
                       rotary_cos=rotary_cos, rotary_sin=rotary_sin, rope_mode=rope_mode, has_mask=True,
-                      block_table=block_table, k_descale=k_descale, v_descale=v_descale)
+                      block_table=block_table, k_descale=k_descale, v_descale=v_descale, _read_table=read_table)
     kv_fp8 = k_cache.dtype == torch.float8_e4m3fn
     seqlen_new, counts = ws.lengths(B, seqlen_k.device)
     if packed:
@@ -1011,7 +1032,9 @@ def fmha_decode_shared_prefix(q, k_cache, v_cache, seqlen_k, block_table, prefix
         ns = _shared_prefix_splits(q.device, B, G, max_group_size, Hq, Hk, sq_max, max(D, Dv), prefix, own)
         num_prefix_splits = num_prefix_splits if num_prefix_splits > 0 else ns[0]
         num_splits = num_splits if num_splits > 0 else ns[1]
-    _debug_validate(seqlen_k=seqlen_k, block_table=block_table, num_total_pages=k_cache.shape[0], page_size=page)
+    if flags.flag("FC_DEBUG_KERNEL_INSTANCE"):
+        validate_paged(seqlen_k=seqlen_k, block_table=_read_entries(block_table, seqlen_k, prefix_lens, cu_groups, max_group_size, page),
+                       num_total_pages=k_cache.shape[0], page_size=page, check=True)
     o = _out("out", out, (*q.shape[:-1], Dv), q.dtype, q)
     if lse is not None:
         _check_tensor("lse", lse, dtype=torch.float32)

@@ -2,12 +2,14 @@
 finite, rows that add nothing, caches with more keys than the weights have columns.
 
 Tolerances are those of test_gpu_key_weights (REL) and test_gpu_shared_prefix (U), derived there."""
+import contextlib
 import math
 
 import pytest
 import torch
 
 import longcontext as lc
+from flashck_amd.utils import flags
 from helpers import dev
 
 pytestmark = pytest.mark.gpu
@@ -121,3 +123,43 @@ def test_a_row_of_nan_is_nan_after_the_merge(fmha, splits):
         assert torch.isnan(got[bad]).all() and torch.isnan(got_lse[bad]).all()
         assert (got.double() - ref[:, 0])[~bad].abs().max() <= (2 * U[torch.float16] + 2.0 ** -20) * 6.0
         assert (got_lse.double() - ref_lse[..., 0])[~bad].abs().max() <= 2e-5
+
+
+@contextlib.contextmanager
+def _checked():
+    flags.set_flag_value("FC_DEBUG_KERNEL_INSTANCE", "true")
+    try:
+        yield
+    finally:
+        flags.set_flag_value("FC_DEBUG_KERNEL_INSTANCE", "false")
+
+
+def test_debug_flag_asks_for_the_entries_that_are_read(fmha):
+    # two groups; rows of sequences other than a group's first hold no page ids for whole pages of the prefix
+    lens, page = [40, 37, 50, 20, 33, 17], 16
+    g = torch.Generator().manual_seed(6)
+    kc, vc, table = lc.pages(g, lens, page, 1, 64, 64, torch.bfloat16)
+    starts, prefixes = [0, 3, 6], [35, 16]
+    lc.share(kc, vc, table, starts, prefixes, page)
+    q = lc.randn(g, 6, 1, 2, 64, dtype=torch.bfloat16)
+    ref, _ = lc.decode(q, kc, vc, lens, table, 0.125)
+    rows = table.clone()
+    rows[1:3, :2] = -1
+    rows[4:, :1] = 10 ** 6
+    args = lambda t: (dev(q), dev(kc), dev(vc), _i32(lens), dev(t), _i32(prefixes))
+    with _checked():
+        o = fmha.fmha_decode_shared_prefix(*args(rows), cu_groups=_i32(starts)).cpu()
+        assert (o.double() - ref).abs().max() <= (2 * U[torch.bfloat16] + 2.0 ** -20) * 6.0
+        for b, j, kw in ((0, 0, {}), (1, 2, {}), (2, 3, {}), (2, 1, dict(max_group_size=2))):
+            bad = rows.clone()
+            bad[b, j] = kc.shape[0]
+            with pytest.raises(ValueError, match=f"first offending sequence: {b}"):
+                fmha.fmha_decode_shared_prefix(*args(bad), cu_groups=_i32(starts), **kw)
+        # a step appends through the sequence's own row: sequence 5 is still inside the prefix of its group
+        short = [40, 37, 50, 20, 33, 15]
+        new = lc.randn(g, 6, 1, 1, 64, dtype=torch.bfloat16)
+        step = lambda t, n: fmha.fmha_decode_step(dev(q), dev(new), dev(new), dev(kc), dev(vc), _i32(n), dev(t), prefix_lens=_i32(prefixes),
+                                                  cu_groups=_i32(starts))
+        step(rows, lens)
+        with pytest.raises(ValueError, match="first offending sequence: 5"):
+            step(rows, short)
