@@ -881,12 +881,12 @@ def fmha_decode_step(q, knew, vnew, k_cache, v_cache, seqlen_k, block_table, *, 
         if q.dim() != 4:
             raise ValueError(f"q must be [B, n, Hq, D] without cu_seqlens_knew, got shape {tuple(q.shape)}")
         n = q.shape[1]
-    read_table = None
+    checked = {}
     if prefix_lens is not None and flags.flag("FC_DEBUG_KERNEL_INSTANCE"):
-        read_table = _read_entries(block_table, seqlen_k, prefix_lens, cu_groups, max_group_size, page, append=True)
+        checked["_read_table"] = _read_entries(block_table, seqlen_k, prefix_lens, cu_groups, max_group_size, page, append=True)
     fmha_fwd_appendkv(q, k_cache, v_cache, knew, vnew, seqlen_k, cu_seqlens_knew=cu_seqlens_knew, max_seqlen_knew=n,
                       rotary_cos=rotary_cos, rotary_sin=rotary_sin, rope_mode=rope_mode, has_mask=True,
-                      block_table=block_table, k_descale=k_descale, v_descale=v_descale, _read_table=read_table)
+                      block_table=block_table, k_descale=k_descale, v_descale=v_descale, **checked)
     kv_fp8 = k_cache.dtype == torch.float8_e4m3fn
     seqlen_new, counts = ws.lengths(B, seqlen_k.device)
     if packed:
