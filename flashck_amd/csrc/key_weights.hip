@@ -15,6 +15,14 @@
 namespace fck {
 namespace {
 
+// keys of a sequence: its count, cut to what its table row (without a table: its row of the cache) holds
+__device__ __forceinline__ int key_count(const KvAddr& a, const KvSeq& s)
+{
+    const int64_t cap = s.table ? (int64_t)a.block_table_stride * a.page_size : a.seqlen_k;
+    const int n = max(s.len, 0);
+    return n < cap ? n : (int)cap;
+}
+
 // K (and Q) tiles are staged in LDS as they lie in memory, rows of ROWB bytes, with the 16-byte chunk index XOR-swizzled by
 // the row so that lanes reading one logical chunk of consecutive rows spread over the banks.
 template <int CH>
@@ -78,7 +86,7 @@ __global__ __launch_bounds__(256) void key_weights_step_kernel(const KeyWeightsA
     const int64_t key0 = (int64_t)(blockIdx.x / a.hk % ranges) * (4 * NT * 32) + wave * (NT * 32);
     if (key0 >= a.cols) return;
     const KvSeq ks = kv_seq(a.kv, b);
-    const int sk = __builtin_amdgcn_readfirstlane(max(ks.len, 0));
+    const int sk = __builtin_amdgcn_readfirstlane(key_count(a.kv, ks));
     const int64_t row_out = ((int64_t)b * a.hk + hkv) * a.cols;
     // tiles that hold keys with a column: what is requested is waited for before the wave ends
     const int64_t key1 = min((int64_t)sk, a.cols);
@@ -319,7 +327,7 @@ __global__ __launch_bounds__(512) void key_weights_window_kernel(const KeyWeight
     int FCK_LDS* const block_full = row_tok + rows32;  // every row of the 32-row block adds something
 
     const KvSeq ks = kv_seq(a.kv, b);
-    const int sk = __builtin_amdgcn_readfirstlane(max(ks.len, 0));
+    const int sk = __builtin_amdgcn_readfirstlane(key_count(a.kv, ks));
     const int tok0 = __builtin_amdgcn_readfirstlane(a.seqstart_q ? a.seqstart_q[b] : b * a.sq);
     const int sq = __builtin_amdgcn_readfirstlane(a.seqstart_q ? a.seqstart_q[b + 1] - tok0 : a.sq);
     const MaskYX mk = make_mask(a.mask_type, a.window_left, a.window_right, sq, sk);
@@ -494,7 +502,7 @@ __global__ __launch_bounds__(512) void key_weights_rows_kernel(const KeyWeightsA
     const int64_t k0 = (int64_t)(part * per_part + in_part) * S::KEYS;
 
     const KvSeq ks = kv_seq(a.kv, b);
-    const int sk = __builtin_amdgcn_readfirstlane(max(ks.len, 0));
+    const int sk = __builtin_amdgcn_readfirstlane(key_count(a.kv, ks));
     const int tok0 = __builtin_amdgcn_readfirstlane(a.seqstart_q ? a.seqstart_q[b] : b * a.sq);
     const int sq = __builtin_amdgcn_readfirstlane(a.seqstart_q ? a.seqstart_q[b + 1] - tok0 : a.sq);
     const MaskYX mk = make_mask(a.mask_type, a.window_left, a.window_right, sq, sk);
@@ -729,7 +737,7 @@ __global__ __launch_bounds__(256) void key_weights_sum_kernel(const KeyWeightsAr
     for (int s = 0; s < a.row_splits; ++s) x += a.partial[s * per + at];
     if (a.weights) {
         const int b = (int)(at / (a.hk * a.cols));
-        if (at % a.cols < kv_seq(a.kv, b).len) x += a.weights[at];
+        if (at % a.cols < key_count(a.kv, kv_seq(a.kv, b))) x += a.weights[at];
     }
     a.out[at] = x;
 }

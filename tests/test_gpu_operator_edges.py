@@ -163,3 +163,22 @@ def test_debug_flag_asks_for_the_entries_that_are_read(fmha):
         step(rows, lens)
         with pytest.raises(ValueError, match="first offending sequence: 5"):
             step(rows, short)
+
+
+@pytest.mark.parametrize("sq,hq,d", [(1, 4, 64), (33, 2, 64), (290, 2, 64)])
+@pytest.mark.parametrize("paged", [True, False])
+def test_counts_beyond_what_the_cache_holds_are_cut(fmha, sq, hq, d, paged):
+    lens, splits = [128, 100], 2 if sq == 290 else 1
+    c = _weights_case(7, lens, sq, hq, 1, d, torch.bfloat16, 64)
+    cache, table = c["kc"], c["table"]
+    if not paged:   # the second sequence's own row ends the tensor
+        cache = torch.stack([torch.nan_to_num(torch.cat([c["kc"][p] for p in table[b].tolist()])) for b in range(2)])
+        c["keys"][1] = cache[1].double()
+    if paged:
+        c["kc"][table[1, 1], 36:] = 0
+        c["keys"][1] = lc.rows(c["kc"], table[1], 128, 64)
+    want = lc.key_weights(c["q"], c["keys"], c["lse"], 300, d ** -0.5, before=torch.ones(2, 1, 300))
+    for n in ([128, 128], [129, 300], [128, 2 ** 31 - 1]):
+        out = fmha.fmha_key_weights(dev(c["q"]), dev(cache), dev(c["lse"]), _i32(n), dev(table) if paged else None,
+                                    weights=dev(torch.ones(2, 1, 300)), num_row_splits=splits)
+        _close(out.cpu(), want, f"{n}")
