@@ -1135,7 +1135,7 @@ int fck_fmha_cache_evict(const void* k_cache, const void* v_cache, void* new_k_c
         return fail(FCK_ERR_INVALID_ARGUMENT, "budget %ld must be positive and hold recent %ld + sinks %ld", (long)budget, (long)recent, (long)sinks);
     if (new_batch_stride_block_table * new_page_block_size < budget)
         return fail(FCK_ERR_INVALID_ARGUMENT, "a row of new_block_table addresses %ld keys, the budget is %ld", (long)(new_batch_stride_block_table * new_page_block_size), (long)budget);
-    if (block_table == new_block_table && k_cache == new_k_cache)
+    if (block_table == new_block_table && (k_cache == new_k_cache || v_cache == new_v_cache))
         return fail(FCK_ERR_INVALID_ARGUMENT, "new_block_table must name other pages than block_table: rows are not moved inside the pages that are read");
     if (!aligned16(workspace)) return fail(FCK_ERR_INVALID_ARGUMENT, "the workspace must be 16-byte aligned");
     if (weights == new_weights) return fail(FCK_ERR_INVALID_ARGUMENT, "new_weights must not be weights");
