@@ -394,6 +394,10 @@ __global__ __launch_bounds__(kThreads) void evict_select_wide_kernel(const Cache
 // that the chain position -> page -> row is walked for all of them at once and 2 kSlots loads are in flight; consecutive
 // threads write consecutive pieces of a slot's row.
 constexpr int kSlots = 4;
+
+// rows of an odd number of 8-byte pieces (an e4m3 cache with such a head dim) are moved 8 bytes at a time
+int move_piece(const CacheEvictArgs& a) { return a.k_row % 16 == 0 && a.v_row % 16 == 0 ? 16 : 8; }
+
 template <typename Piece>
 __global__ __launch_bounds__(256) void evict_move_kernel(const CacheEvictArgs a)
 {
@@ -440,14 +444,19 @@ __global__ __launch_bounds__(256) void evict_move_kernel(const CacheEvictArgs a)
 template <typename Piece>
 hipError_t launch_move(const CacheEvictArgs& a, hipStream_t st)
 {
-    const int64_t pieces = (a.k_row > a.v_row ? a.k_row : a.v_row) / (int)sizeof(Piece);
-    const int64_t items = (int64_t)a.batch * ((a.budget + kSlots - 1) / kSlots) * a.hk * pieces;
-    if (items > INT32_MAX) return hipErrorInvalidValue;
+    const int64_t items = cache_evict_move_items(a);
     hipLaunchKernelGGL((evict_move_kernel<Piece>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
 }  // namespace
+
+int64_t cache_evict_move_items(const CacheEvictArgs& a)
+{
+    const int64_t pieces = (a.k_row > a.v_row ? a.k_row : a.v_row) / move_piece(a);
+    const int64_t groups = ((int64_t)a.budget + kSlots - 1) / kSlots * pieces, rows = (int64_t)a.batch * a.hk;
+    return rows > INT32_MAX / groups ? -1 : rows * groups;  // the kernel counts in 32 bits
+}
 
 size_t cache_evict_workspace_bytes(int64_t rows, int64_t cols, int num_cu)
 {
@@ -469,8 +478,7 @@ hipError_t launch_cache_evict(const CacheEvictArgs& a, hipStream_t st)
         hipLaunchKernelGGL(evict_select_kernel, rows, threads, 0, st, a);
     }
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    // rows of an odd number of 8-byte pieces (an e4m3 cache with such a head dim) are moved 8 bytes at a time
-    return a.k_row % 16 == 0 && a.v_row % 16 == 0 ? launch_move<u32x4_t>(a, st) : launch_move<u32x2_t>(a, st);
+    return move_piece(a) == 16 ? launch_move<u32x4_t>(a, st) : launch_move<u32x2_t>(a, st);
 }
 
 }  // namespace fck

@@ -1133,6 +1133,10 @@ int fck_fmha_cache_evict(const void* k_cache, const void* v_cache, void* new_k_c
     if (int rc = check_fit32(batch, hk, cols, budget, page_block_size, batch_stride_block_table, new_page_block_size, new_batch_stride_block_table, batch * hk)) return rc;
     if (budget <= 0 || recent < 0 || sinks < 0 || recent > budget || sinks > budget - recent)
         return fail(FCK_ERR_INVALID_ARGUMENT, "budget %ld must be positive and hold recent %ld + sinks %ld", (long)budget, (long)recent, (long)sinks);
+    // the kernels step through a row by strides of up to 8192 in 32 bits
+    constexpr int64_t kMostKeys = (int64_t)1 << 30;
+    if (budget > kMostKeys || batch_stride_block_table * page_block_size > kMostKeys)
+        return fail(FCK_ERR_UNSUPPORTED, "budget %ld, %ld keys per row of block_table: at most 2^30", (long)budget, (long)(batch_stride_block_table * page_block_size));
     if (new_batch_stride_block_table * new_page_block_size < budget)
         return fail(FCK_ERR_INVALID_ARGUMENT, "a row of new_block_table addresses %ld keys, the budget is %ld", (long)(new_batch_stride_block_table * new_page_block_size), (long)budget);
     if (block_table == new_block_table && (k_cache == new_k_cache || v_cache == new_v_cache))
@@ -1170,6 +1174,8 @@ int fck_fmha_cache_evict(const void* k_cache, const void* v_cache, void* new_k_c
     a.workspace = workspace && fck::cache_evict_workspace_bytes(batch * hk, cols, cu_count()) > 0 ? workspace : nullptr;
     a.k_row = (int32_t)(d * e);
     a.v_row = (int32_t)(dv * e);
+    if (fck::cache_evict_move_items(a) < 0)
+        return fail(FCK_ERR_INVALID_ARGUMENT, "budget %ld x %ld sequences x %ld heads is more than one move covers", (long)budget, (long)batch, (long)hk);
     g_kernel = "evict_move_kernel";
     return launch_status(fck::launch_cache_evict(a, static_cast<hipStream_t>(stream)), "cache eviction launch");
 }

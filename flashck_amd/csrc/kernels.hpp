@@ -193,6 +193,8 @@ struct CacheEvictArgs {
 };
 // bytes of workspace with which the choice of `rows` rows of `cols` weights is spread over the chip; 0: it is not worth it
 size_t cache_evict_workspace_bytes(int64_t rows, int64_t cols, int num_cu);
+// threads of the move; -1: more than one launch can have
+int64_t cache_evict_move_items(const CacheEvictArgs& a);
 hipError_t launch_cache_evict(const CacheEvictArgs& a, hipStream_t st);
 
 // arguments of the paged-cache checker: a block table (block_table != nullptr: seqlen_k, block_table_stride) or a page
