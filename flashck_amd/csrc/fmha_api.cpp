@@ -941,12 +941,14 @@ int fck_fmha_shared_prefix_splits(int64_t batch, int64_t num_groups, int64_t max
     // The items (a split x a KV head x a row tile) of the longest prefixes and of half the longest own keys make two equal ones
     // per CU.  The small kernels leave room for three, but more partial results to merge cost more than that gives: 32 sequences
     // on 4096 shared and up to 1024 own keys took 30 us with 16 + 4 splits (three per CU), 26 us with 11 + 3, 27 us with 10 + 2.
-    const int64_t rows = max_group_size * sq * (hq / hk);
+    const double packed = (double)max_group_size * sq * (hq / hk);
+    if (packed > INT32_MAX || (double)sq * (hq / hk) > INT32_MAX) return FCK_OK;
+    const int64_t rows = (int64_t)packed;
     const int d = kernel_dim(head_dim, head_dim), bm = 64 * fck::shared_prefix_blocks(d, rows);
     const double slots = 2.0 * (num_cu > 0 ? (double)num_cu : cu_count());
     const auto tiles = [&](int64_t r) { return (double)((r + bm - 1) / bm); };
     const double prefix = max_prefix_len > 0 ? (double)max_prefix_len : 0, own = max_own_len > 0 ? (double)max_own_len : 0;
-    const double keys = (double)hk * (num_groups * tiles(rows) * prefix + batch * tiles(sq * (hq / hk)) * own / 2);
+    const double keys = (double)hk * ((double)num_groups * tiles(rows) * prefix + batch * tiles(sq * (hq / hk)) * own / 2);
     const double chunk = std::fmax(64.0, std::ceil(keys / slots / 64) * 64);
     const auto splits = [&](double n) { return (int32_t)std::fmin(64.0, std::fmax(1.0, std::ceil(n / chunk))); };
     if (prefix_splits) *prefix_splits = splits(prefix);
@@ -972,13 +974,19 @@ int fck_fmha_decode_shared_prefix(const void* q, const void* k_cache, const void
         return fail(FCK_ERR_INVALID_ARGUMENT, "q, k_cache, v_cache, o and o_acc must be 16-byte aligned");
     if (!(scale > 0.f) || !std::isfinite(scale)) return fail(FCK_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
     if (seqlen_q <= 0) return fail(FCK_ERR_INVALID_ARGUMENT, "seqlen_q must be positive (group mode: it carries total_q)");
-    if (q_max_seq_len <= 0) q_max_seq_len = seqlen_q;
+    if (q_max_seq_len <= 0 || q_max_seq_len > seqlen_q) q_max_seq_len = seqlen_q;
     if (num_groups < 1 || (!cu_groups && num_groups != 1)) return fail(FCK_ERR_INVALID_ARGUMENT, "num_groups must be positive, and 1 without cu_groups");
     if (max_group_size <= 0 || max_group_size > batch) max_group_size = batch;
     if (num_prefix_splits < 1 || num_prefix_splits > 64 || num_own_splits < 1 || num_own_splits > 64)
         return fail(FCK_ERR_INVALID_ARGUMENT, "num_prefix_splits %ld / num_own_splits %ld out of range [1,64]", (long)num_prefix_splits, (long)num_own_splits);
     if (page_block_size <= 0 || batch_stride_block_table <= 0) return fail(FCK_ERR_INVALID_ARGUMENT, "page_block_size and batch_stride_block_table must be positive");
-    if (int rc = check_fit32(page_block_size, batch_stride_block_table, seqlen_q, q_max_seq_len, num_groups, (seqstart_q ? 1 : batch) * seqlen_q)) return rc;
+    if (int rc = check_fit32(page_block_size, batch_stride_block_table, seqlen_q, num_groups, (seqstart_q ? 1 : batch) * seqlen_q)) return rc;
+    // packed rows of a sequence and of a group (packed queries: never more than there are)
+    int64_t tokens = max_group_size * q_max_seq_len;
+    if (seqstart_q && tokens > seqlen_q) tokens = seqlen_q;
+    const int64_t g = hq / hk;
+    if (int rc = check_fit32(tokens)) return rc;
+    if (int rc = check_fit32(q_max_seq_len * g, tokens * g, batch * hk, num_groups * hk)) return rc;
     // keys per split; what lies behind the bounds goes to the last split
     const int64_t capacity = batch_stride_block_table * page_block_size;
     const auto chunk = [&](int64_t bound, int64_t ns) {
@@ -1025,9 +1033,8 @@ int fck_fmha_decode_shared_prefix(const void* q, const void* k_cache, const void
     if (a.mod.bias_type == FCK_BIAS_ELEMENTWISE) return fail(FCK_ERR_UNSUPPORTED, "shared-prefix decode takes ALiBi and the soft cap, not an elementwise bias");
     if (int rc = only_score_attrs(attrs)) return rc;
     if (int rc = fill_cache_type(a.kv8, a.scale_log2, a.mod, &a.v_descale, attrs, d, dv)) return rc;
-    const int64_t g = hq / hk;
     g_kernel = "shared_prefix_kernel";
-    return launch_status(fck::launch_shared_prefix(a, kernel_dim(d, dv), dtype, max_group_size * q_max_seq_len * g, q_max_seq_len * g,
+    return launch_status(fck::launch_shared_prefix(a, kernel_dim(d, dv), dtype, tokens * g, q_max_seq_len * g,
                                                    static_cast<hipStream_t>(stream)), "shared-prefix decode launch");
 }
 
@@ -1037,7 +1044,7 @@ int fck_fmha_key_weights_row_splits(int64_t batch, int64_t hq, int64_t hk, int64
     for (int64_t v : {batch, hq, hk, d})
         if (v <= 0 || v > kMax) return 1;
     if (hk > hq || d > 256 || sq <= 0 || sq > INT32_MAX || cols <= 0 || cols > INT32_MAX || num_cu > kMax) return 1;
-    if (batch * hk > INT32_MAX) return 1;
+    if (batch * hk > INT32_MAX || sq * (hq / hk) > INT32_MAX) return 1;
     return fck::key_weights_row_splits(kernel_dim(d, d), batch, hk, hq / hk, sq, cols, mask_type != 0, num_cu > 0 ? (int)num_cu : cu_count());
 }
 
@@ -1056,9 +1063,9 @@ int fck_fmha_key_weights(const void* q, const void* k, const void* lse, const vo
     if (!(scale > 0.f) || !std::isfinite(scale)) return fail(FCK_ERR_INVALID_ARGUMENT, "scale must be positive and finite");
     if (seqlen_q <= 0) return fail(FCK_ERR_INVALID_ARGUMENT, "seqlen_q must be positive (group mode: it carries total_q)");
     if (cols <= 0) return fail(FCK_ERR_INVALID_ARGUMENT, "cols (keys a row of the weights holds) must be positive");
-    if (q_max_seq_len <= 0) q_max_seq_len = seqlen_q;
-    if (int rc = check_fit32(seqlen_q, seqlen_k, q_max_seq_len, cols, batch_stride_block_table, page_block_size, (seqstart_q ? 1 : batch) * seqlen_q,
-                             q_max_seq_len * (hq / hk))) return rc;
+    if (q_max_seq_len <= 0 || q_max_seq_len > seqlen_q) q_max_seq_len = seqlen_q;
+    if (int rc = check_fit32(seqlen_q, seqlen_k, cols, batch_stride_block_table, page_block_size, (seqstart_q ? 1 : batch) * seqlen_q, batch * hk)) return rc;
+    if (int rc = check_fit32(q_max_seq_len * (hq / hk))) return rc;
     if (num_row_splits < 1 || num_row_splits > 16) return fail(FCK_ERR_INVALID_ARGUMENT, "num_row_splits %ld out of range [1,16]", (long)num_row_splits);
     if (num_row_splits > 1 && !workspace) return fail(FCK_ERR_INVALID_ARGUMENT, "num_row_splits > 1 needs a workspace");
     fck::KeyWeightsArgs a{};
@@ -1108,7 +1115,7 @@ int fck_fmha_key_weights(const void* q, const void* k, const void* lse, const vo
 
 size_t fck_fmha_cache_evict_workspace_bytes(int64_t batch, int64_t hk, int64_t cols, int64_t num_cu)
 {
-    if (batch <= 0 || hk <= 0 || cols <= 0 || batch > INT32_MAX || hk > INT32_MAX || num_cu > INT32_MAX) return 0;
+    if (batch <= 0 || hk <= 0 || cols <= 0 || batch > INT32_MAX || hk > INT32_MAX || batch * hk > INT32_MAX || num_cu > INT32_MAX) return 0;
     return fck::cache_evict_workspace_bytes(batch * hk, cols, num_cu > 0 ? (int)num_cu : cu_count());
 }
 

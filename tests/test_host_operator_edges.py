@@ -34,3 +34,44 @@ def test_abi_eviction_refuses_what_it_cannot_move_before_it_chooses(sizes):
 def test_abi_eviction_refuses_rows_beyond_its_counters():
     assert _abi_evict(budget=(1 << 31) - 1, dtype=1, d=8, dv=8, hk=1, batch=1, npage=1 << 10, nstride=1 << 21) == -2
     assert _abi_evict(stride=(1 << 20) + 1, page=1 << 10) == -2
+
+
+def _abi_shared(**kw):
+    a = dict(q=_at(1), k=_at(2), v=_at(3), o=_at(4), lse=None, lse_acc=_at(5), o_acc=_at(6), sq_start=_at(7), sk=_at(8), bt=_at(9), cu=_at(10), pl=_at(11),
+             batch=2, groups=1, gmax=0, sq=2, hq=4, hk=2, d=64, dv=64, qmax=1, nsp=1, nso=1, maxp=0, maxo=0, stride=2, page=16, scale=0.1, wl=-1,
+             wr=-1, mask=0, dtype=4, attrs=None, stream=None)
+    a.update(kw)
+    return _lib.load().fck_fmha_decode_shared_prefix(*a.values())
+
+
+def _abi_weights(**kw):
+    a = dict(q=_at(1), k=_at(2), lse=_at(3), w=None, out=_at(4), ws=None, sq_start=_at(5), sk=_at(6), bt=_at(7), stride=2, page=16, batch=2, sq=2, skc=0,
+             cols=32, hq=4, hk=2, d=64, qmax=1, ns=1, scale=0.1, wl=-1, wr=-1, mask=0, dtype=4, attrs=None, stream=None)
+    a.update(kw)
+    return _lib.load().fck_fmha_key_weights(*a.values())
+
+
+@pytest.mark.parametrize("call,sizes", [
+    (_abi_shared, dict(batch=1 << 22, sq=1 << 30, qmax=1 << 30, hq=1 << 11, hk=1)),   # rows of a group: 2^63
+    (_abi_shared, dict(batch=1 << 22, sq=1 << 30, qmax=1 << 30, hq=1 << 12, hk=1)),   # 2^64
+    (_abi_shared, dict(batch=1 << 30, hq=1 << 30, hk=1 << 30)),
+    (_abi_shared, dict(groups=1 << 30, hq=1 << 30, hk=1 << 30)),
+    (_abi_weights, dict(batch=1 << 30, hq=1 << 30, hk=1 << 30, cols=1 << 30)),
+    (_abi_weights, dict(sq=1 << 30, qmax=1 << 30, hq=1 << 30, hk=1)),
+])
+def test_abi_sizes_whose_products_leave_64_bits_are_refused(call, sizes):
+    assert call(**sizes) == -1
+    assert b"beyond 32 bits" in _lib.load().fck_last_error()
+
+
+def test_abi_choices_for_sizes_whose_products_leave_64_bits():
+    lib = _lib.load()
+    a, b = ctypes.c_int32(), ctypes.c_int32()
+    most = 1 << 24
+    for sizes in ((most, most, most, most, 1, most), (1, 1, most, most, 1, 1 << 16), (1, 1, 1, 1, 1, most), (most, most, most, most, most, most)):
+        assert lib.fck_fmha_shared_prefix_splits(*sizes, 128, 1 << 20, 1 << 20, 256, ctypes.byref(a), ctypes.byref(b)) == 0
+        assert 1 <= a.value <= 64 and 1 <= b.value <= 64, sizes
+    for sizes in ((1, most, 1, (1 << 31) - 1, 1 << 20, 256), (1, most, 1, 1 << 30, (1 << 31) - 1, 64)):
+        assert lib.fck_fmha_key_weights_row_splits(*sizes, 2, 256) == 1, sizes
+    assert lib.fck_fmha_cache_evict_workspace_bytes(1 << 30, 1 << 30, 1 << 20, 256) == 0
+    assert lib.fck_fmha_cache_evict_workspace_bytes((1 << 31) - 1, (1 << 31) - 1, 1 << 20, 256) == 0
