@@ -250,8 +250,9 @@ __global__ __launch_bounds__(256, (kSharedWaves<D, MB>)) void shared_prefix_kern
 #pragma unroll
         for (int u = 0; u < S::LD; ++u) {
             const int row = (u * 256 + tid) / S::CH, chunk = (u * 256 + tid) % S::CH;
-            // rows outside the item's keys repeat its first or last one (their scores are masked)
-            const int key = min(max(kb + row, key_lo), key_hi - 1);
+            // Rows outside the walked keys repeat the first or last of them: their scores are masked, but a probability of 0 times
+            // an infinite or NaN value is NaN, so a key that no row of the workgroup sees must not be read either.
+            const int key = min(max(kb + row, vis_lo), vis_hi - 1);
             const int64_t cr = kUniform ? row0 + (key - kb) : cache_row(key);
             kreg[u] = fetch(a.k, cr, chunk, dq);
             vreg[u] = fetch(a.v, cr, chunk, dvs);

@@ -182,3 +182,25 @@ def test_counts_beyond_what_the_cache_holds_are_cut(fmha, sq, hq, d, paged):
         out = fmha.fmha_key_weights(dev(c["q"]), dev(cache), dev(c["lse"]), _i32(n), dev(table) if paged else None,
                                     weights=dev(torch.ones(2, 1, 300)), num_row_splits=splits)
         _close(out.cpu(), want, f"{n}")
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+@pytest.mark.parametrize("sq,page,window,prefix", [(1, 64, (20, 0), 0), (1, 16, (20, 0), 90), (3, 64, (30, 2), 70), (1, 128, (0, 0), 100), (2, 48, (150, 0), 40)])
+def test_values_of_keys_outside_the_window_do_not_matter(fmha, bad, sq, page, window, prefix):
+    lens = [prefix + 30, prefix + 101]
+    c = _shared_case(8, lens, prefix, sq, 4, 2, 64, torch.bfloat16, page)
+    for b, n in enumerate(lens):
+        for t in range(max(0, n - sq - window[0])):
+            # a key of the prefix may be in the other sequence's window
+            if t >= prefix or t < min(lens) - sq - window[0]:
+                for pool in (c["kc"], c["vc"]):
+                    pool[c["table"][b, t // page], t % page] = bad
+    kw = dict(mask_type=2, window=window)
+    ref, ref_lse = lc.decode(c["q"], c["kc"], c["vc"], lens, c["table"], 0.125, **kw)
+    lse = dev(torch.zeros(2, 4, sq))
+    for splits in ((1, 1), (3, 2)):
+        o = fmha.fmha_decode_shared_prefix(dev(c["q"]), dev(c["kc"]), dev(c["vc"]), _i32(lens), dev(c["table"]), _i32([prefix]), lse=lse,
+                                           num_prefix_splits=splits[0], num_splits=splits[1], **kw).cpu()
+        assert torch.isfinite(o.float()).all()
+        assert (o.double() - ref).abs().max() <= (2 * U[torch.bfloat16] + 2.0 ** -20) * 6.0
+        assert (lse.cpu().double() - ref_lse).abs().max() <= 2e-5
