@@ -987,16 +987,18 @@ int fck_fmha_decode_shared_prefix(const void* q, const void* k_cache, const void
     const int64_t g = hq / hk;
     if (int rc = check_fit32(tokens)) return rc;
     if (int rc = check_fit32(q_max_seq_len * g, tokens * g, batch * hk, num_groups * hk)) return rc;
-    // keys per split; what lies behind the bounds goes to the last split
+    // Fewest keys per split: the equal parts of the bound, but never more than `most`, which is what a loose bound comes to.
+    // 32 sequences on 4096 shared keys, bounds of 131072: 31 us with 256 for the prefix, 34 us with 128; 4 sequences on 512 shared
+    // keys, bounds of 32768: 17.5 and 15 us.  Own keys, exact bounds, the first batch: 25.2 us with 256, 25.8 us with 128.
     const int64_t capacity = batch_stride_block_table * page_block_size;
-    const auto chunk = [&](int64_t bound, int64_t ns) {
+    const auto chunk = [&](int64_t bound, int64_t ns, int64_t most) {
         if (bound <= 0 || bound > capacity) bound = capacity;
         const int64_t c = ((bound + ns - 1) / ns + 63) / 64 * 64;
-        return (int32_t)(c > INT32_MAX / 64 * 64 ? INT32_MAX / 64 * 64 : c);
+        return (int32_t)(c > most ? most : c);
     };
     fck::SharedPrefixArgs a{};
-    a.prefix_chunk = chunk(max_prefix_len, num_prefix_splits);
-    a.own_chunk = chunk(max_own_len, num_own_splits);
+    a.prefix_chunk = chunk(max_prefix_len, num_prefix_splits, 128);
+    a.own_chunk = chunk(max_own_len, num_own_splits, 256);
     a.q = q;
     a.k = k_cache;
     a.v = v_cache;

@@ -128,7 +128,7 @@ struct SharedPrefixArgs {
     int32_t batch, groups, max_group;  // max_group: sequences of a group the prefix rows cover (the others read all of their own keys)
     int32_t sq, hq, hk, d, dv;
     int32_t ns_prefix, ns_own;
-    int32_t prefix_chunk, own_chunk;  // keys per split (multiples of 64)
+    int32_t prefix_chunk, own_chunk;  // fewest keys per split (multiples of 64)
     int32_t prefix_tiles, own_tiles;  // row tiles per (group, KV head) / per (sequence, KV head); set by the launcher
     int32_t prefix_items;             // workgroups that handle prefixes; set by the launcher
     int64_t shape_sq;                 // Sq of the workspace: sq (batch mode) or total_q

@@ -152,10 +152,13 @@ __global__ __launch_bounds__(256, (kSharedWaves<D, MB>)) void shared_prefix_kern
     const int64_t R = (int64_t)(tok1 - tok0) * g;
     const int64_t r0 = (int64_t)mt * S::BM;
     if (r0 >= R) return;
-    // A split is a chunk of whole tiles, the same for every group or sequence: items of one size pack better than equal parts of
-    // ragged lengths.  The last one takes whatever lies behind the caller's bound; a short sequence leaves its last ones empty.
+    // A split is an equal part of the keys there are, in whole tiles, and no smaller than the caller's least chunk (which leaves
+    // the last splits of a short range empty).  Parts sized from host bounds alone put a range beyond its bound into the last
+    // split, and everything into the first when the bound is loose: 32 sequences on 4096 shared keys with bounds of 32768 took
+    // 96 us (32 us so; with exact bounds 25 us either way).
     const int base = key_lo / S::TK * S::TK;
-    const int64_t per = prefix ? a.prefix_chunk : a.own_chunk;
+    const int64_t part = ((int64_t)key_hi - base + ns - 1) / ns;
+    const int64_t per = max((int64_t)(prefix ? a.prefix_chunk : a.own_chunk), (part + 63) / 64 * 64);
     const int k0 = (int)min(max((int64_t)key_lo, base + per * split), (int64_t)key_hi);
     const int k1 = split == ns - 1 ? key_hi : (int)min((int64_t)key_hi, base + per * (split + 1));
 

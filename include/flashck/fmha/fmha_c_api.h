@@ -291,8 +291,9 @@ FCK_EXPORT int fck_fmha_fwd_splitkv_combine_lse(const void* lse_acc, const void*
  *   max_group_size  at most this many sequences of a group share (0: batch); the ones behind read all their own keys
  *   seqlen_k_ptr  int32 [B], key counts with the prefix
  *   q, o, lse     as fck_fmha_fwd_splitkv and its combine; seqlen_q carries total_q in group mode; lse may be NULL
- *   max_prefix_len, max_own_len  the longest prefix and the most keys a sequence has behind it (0: what the table can address):
- *                 a split holds ceil(bound / splits) keys rounded up to 64, the last one whatever lies behind the bound
+ *   max_prefix_len, max_own_len  the longest prefix and the most keys a sequence has behind it (0: what the table can address).
+ *                 The keys there are (of a prefix, of a sequence behind it) are cut into equal parts, one per split, rounded up
+ *                 to 64; these bounds only say how small a part may be: ceil(bound / splits), at most 128 (prefix) or 256 keys
  *   o_acc, lse_acc  fp32 workspace [Bs, Hq, num_prefix_splits + num_own_splits, Sq, Dv] and without Dv
  *                 (fck_fmha_splitkv_workspace_bytes); split counts in [1, 64], fck_fmha_shared_prefix_splits chooses them
  * attrs: ALiBi, soft cap, kv_dtype with its scales.  Two launches.  A row whose mask leaves no key gets zeros and lse -inf;

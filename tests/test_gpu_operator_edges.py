@@ -204,3 +204,22 @@ def test_values_of_keys_outside_the_window_do_not_matter(fmha, bad, sq, page, wi
         assert torch.isfinite(o.float()).all()
         assert (o.double() - ref).abs().max() <= (2 * U[torch.bfloat16] + 2.0 ** -20) * 6.0
         assert (lse.cpu().double() - ref_lse).abs().max() <= 2e-5
+
+
+@pytest.mark.parametrize("bounds", [dict(), dict(max_prefix_len=30000, max_seqlen_k=30000), dict(max_prefix_len=64, max_seqlen_k=128)])
+def test_every_split_takes_its_part_of_the_keys_whatever_the_bounds(fmha, bounds):
+    # a table that can address far more than the sequences have, bounds far above and below what they have
+    lens, prefix, nsp, nso = [2048 + 1100, 2048 + 1024, 2048 + 10], 2048, 8, 4
+    c = _shared_case(9, lens, prefix, 1, 2, 1, 64, torch.bfloat16, 64)
+    table = torch.cat([c["table"], torch.zeros(3, 600, dtype=torch.int32)], dim=1)
+    ws = fmha.DecodeWorkspace()
+    lse = dev(torch.zeros(3, 2, 1))
+    o = fmha.fmha_decode_shared_prefix(dev(c["q"]), dev(c["kc"]), dev(c["vc"]), _i32(lens), dev(table), _i32([prefix]), lse=lse, workspace=ws,
+                                       num_prefix_splits=nsp, num_splits=nso, **bounds)
+    _, parts = ws.partials(3, 2, nsp + nso, 1, 64, o.device)
+    some = torch.isfinite(parts.cpu())[..., 0]
+    assert some[:, :, :nsp].all() and some[:2, :, nsp:].all()
+    assert some[2, :, nsp].all() and not some[2, :, nsp + 1:].any()   # 10 keys are not cut
+    ref, ref_lse = lc.decode(c["q"], c["kc"], c["vc"], lens, c["table"], 0.125)
+    assert (o.cpu().double() - ref).abs().max() <= (2 * U[torch.bfloat16] + 2.0 ** -20) * 6.0
+    assert (lse.cpu().double() - ref_lse).abs().max() <= 2e-5

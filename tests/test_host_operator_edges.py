@@ -2,8 +2,10 @@
 import ctypes
 
 import pytest
+import torch
 
 from flashck_amd import _lib
+from flashck_amd.ops.fmha import fmha as F
 
 
 def _at(n):
@@ -75,3 +77,29 @@ def test_abi_choices_for_sizes_whose_products_leave_64_bits():
         assert lib.fck_fmha_key_weights_row_splits(*sizes, 2, 256) == 1, sizes
     assert lib.fck_fmha_cache_evict_workspace_bytes(1 << 30, 1 << 30, 1 << 20, 256) == 0
     assert lib.fck_fmha_cache_evict_workspace_bytes((1 << 31) - 1, (1 << 31) - 1, 1 << 20, 256) == 0
+
+
+def test_default_splits_hold_for_a_sequence_without_the_prefix():
+    # B, groups, group size, Hq, Hk, tokens, head dim; longest prefix, keys behind it, longest sequence
+    for sizes in ((32, 2, 32, 32, 8, 1, 128), (4, 1, 4, 32, 8, 1, 128), (8, 2, 4, 16, 4, 1, 64), (64, 1, 64, 64, 8, 1, 128), (24, 3, 24, 16, 4, 4, 64)):
+        batch, _, _, hq, hk, sq, d = sizes
+        for prefix, own, longest in ((32768, 232, 33000), (32768, 1, 32768), (512, 64, 576), (1, 4096, 4097)):
+            ns = F._default_shared_prefix_splits(*sizes, prefix, own, longest)
+            assert all(1 <= n <= 64 for n in ns)
+            alone = F.num_splits_heuristic(batch, hq, hk, sq, longest, d)
+            assert ns[1] >= min(alone, -(-longest // 2048)), (sizes, prefix, own, longest, ns)
+
+
+def test_missing_bounds_leave_the_prefix_its_splits(monkeypatch):
+    seen, call = [], F._call
+    monkeypatch.setattr(F, "_REQUIRE_GPU_TENSORS", False)
+    monkeypatch.setattr(F, "_stream", lambda: None)
+    monkeypatch.setattr(F, "_call", lambda name, *args: seen.append(args) if name == "fck_fmha_decode_shared_prefix" else call(name, *args))
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)
+    cache = torch.zeros(1, 128, 8, 128, dtype=torch.bfloat16)
+    for pages in (64, 256, 1024):
+        F.fmha_decode_shared_prefix(torch.zeros(32, 1, 32, 128, dtype=torch.bfloat16), cache, cache, i32(*[5000] * 32),
+                                    torch.zeros(32, pages, dtype=torch.int32), i32(4096))
+        args = seen[-1]
+        # one group of 128 packed rows and 8 KV heads: as many prefix splits as make its items fill the chip, whatever the table addresses
+        assert args[21] >= 16 and args[22] >= 2, args[21:23]
