@@ -1,6 +1,6 @@
 """Which kernel instantiations of the device build does the test suite launch?
 
-    python tests/emu/kernel_coverage.py            # runs the emulator suite (about ten minutes), then reports
+    python tests/emu/kernel_coverage.py            # runs the emulator suites (about twenty minutes), then reports
     python tests/emu/kernel_coverage.py FILE ...   # reports on coverage files written earlier (EMU_COVERAGE=FILE)
 
 The kernels are templates; a library of 300 instantiations can pass every test with a third of them never run.  The
@@ -20,6 +20,7 @@ ROOT = os.path.dirname(os.path.dirname(HERE))
 sys.path.insert(0, ROOT)
 
 # without the six prefill cases that are hours of emulation each (they launch nothing the others do not)
+SUITES = ["test_emu_kernels.py", "test_emu_operators.py", "test_emu_operator_edges.py"]
 SLOW = "not workload5_full and not midsize_every_row and not large_pool and not longer_than_the_page_cache"
 
 
@@ -29,6 +30,7 @@ def _demangle(names, types=False):
 
 
 def _norm(name):
+    name = name.replace("(anonymous namespace)::", "")
     name = re.sub(r"\(.*\)$", "", name.replace("void ", "").strip())   # no return type, no parameter list
     return re.sub(r"\s+", "", re.sub(r"\b\w+::", "", name))            # no namespaces, no blanks
 
@@ -65,8 +67,8 @@ def main(argv):
     if not files:
         fd, path = tempfile.mkstemp(suffix=".cov")
         os.close(fd)
-        env = dict(os.environ, EMU_COVERAGE=path, FCK_EMU_FULL="1")
-        cmd = [sys.executable, "-m", "pytest", os.path.join(ROOT, "tests", "test_emu_kernels.py"), "-q", "-n", "6", "-k", SLOW]
+        env = dict(os.environ, EMU_COVERAGE=path, FCK_EMU_FULL="1", OMP_NUM_THREADS="1")   # the workers share the cores
+        cmd = [sys.executable, "-m", "pytest", *[os.path.join(ROOT, "tests", s) for s in SUITES], "-q", "-n", "6", "-k", SLOW]
         r = subprocess.run(cmd, env=env, cwd=ROOT)
         if r.returncode != 0:
             return r.returncode
