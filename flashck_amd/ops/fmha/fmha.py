@@ -812,20 +812,32 @@ class DecodeWorkspace:
     """Buffers a decode step needs besides its inputs and outputs, kept between steps.
 
     Holds the split-KV partials (o_acc, lse_acc) and the advanced key counts.  Buffers are only reallocated when a
-    step needs a larger one, so a serving loop with a fixed batch allocates on its first step only.
+    step needs a larger one, so a serving loop with a fixed batch allocates on its first step only.  A buffer that was outgrown
+    stays allocated as long as the workspace: a graph captured with it writes to it at every replay.  One workspace serves one
+    stream at a time.
     """
 
     def __init__(self):
+        self._outgrown = []
         self._o_acc = None
         self._lse_acc = None
         self._seqlen = None
         self._counts = None
 
-    @staticmethod
-    def _fit(buf, numel, dtype, device):
-        if buf is None or buf.numel() < numel or buf.dtype != dtype or buf.device != device:
-            buf = torch.empty(numel, dtype=dtype, device=device)
-        return buf
+    def _fit(self, buf, numel, dtype, device):
+        fits = lambda x: x.numel() >= numel and x.dtype == dtype and x.device == device
+        if buf is None:
+            return torch.empty(numel, dtype=dtype, device=device)
+        if fits(buf):
+            return buf
+        self._outgrown.append(buf)
+        for i, old in enumerate(self._outgrown):
+            if fits(old):
+                return self._outgrown.pop(i)
+        # half as much again at least: what was outgrown then adds up to less than twice the buffer in use
+        if buf.dtype == dtype and buf.device == device:
+            numel = max(numel, buf.numel() * 3 // 2)
+        return torch.empty(numel, dtype=dtype, device=device)
 
     def partials(self, shape_batch, q_num_heads, num_splits, shape_seqlen_q, v_head_dim, device):
         n_lse = shape_batch * q_num_heads * num_splits * shape_seqlen_q

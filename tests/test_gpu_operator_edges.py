@@ -223,3 +223,24 @@ def test_every_split_takes_its_part_of_the_keys_whatever_the_bounds(fmha, bounds
     ref, ref_lse = lc.decode(c["q"], c["kc"], c["vc"], lens, c["table"], 0.125)
     assert (o.cpu().double() - ref).abs().max() <= (2 * U[torch.bfloat16] + 2.0 ** -20) * 6.0
     assert (lse.cpu().double() - ref_lse).abs().max() <= 2e-5
+
+
+def test_a_captured_call_survives_a_workspace_that_grows(fmha):
+    c = _shared_case(10, [200, 220], 150, 1, 4, 2, 64, torch.bfloat16, 64)
+    big = _shared_case(11, [300] * 12, 150, 1, 4, 2, 64, torch.bfloat16, 64)
+    inputs = lambda x: (dev(x["q"]), dev(x["kc"]), dev(x["vc"]), _i32(x["lens"]), dev(x["table"]), _i32([150]))
+    args, more = inputs(c), inputs(big)
+    ws, out = fmha.DecodeWorkspace(), torch.empty_like(args[0])
+    want = fmha.fmha_decode_shared_prefix(*args)
+    fmha.fmha_decode_shared_prefix(*args, workspace=ws, out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        fmha.fmha_decode_shared_prefix(*args, workspace=ws, out=out)
+    fmha.fmha_decode_shared_prefix(*more, workspace=ws)   # outgrows the buffers of the graph
+    others = [torch.full((n,), 7.0, device="cuda") for n in (256, 1024, 4096, 16384, 65536) for _ in range(8)]   # would take their place
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and all((x == 7.0).all() for x in others)

@@ -103,3 +103,23 @@ def test_missing_bounds_leave_the_prefix_its_splits(monkeypatch):
         args = seen[-1]
         # one group of 128 packed rows and 8 KV heads: as many prefix splits as make its items fill the chip, whatever the table addresses
         assert args[21] >= 16 and args[22] >= 2, args[21:23]
+
+
+def test_an_outgrown_workspace_buffer_stays_allocated():
+    # a graph captured with the smaller buffers goes on writing to them
+    import gc
+    import weakref
+    ws, device = F.DecodeWorkspace(), torch.device("cpu")
+    ws.partials(2, 4, 3, 1, 64, device)
+    ws.lengths(2, device)
+    old = [weakref.ref(x) for x in (ws._o_acc, ws._lse_acc, ws._seqlen)]
+    o, lse = ws.partials(2, 4, 9, 1, 64, device)
+    ws.lengths(5, device)
+    gc.collect()
+    assert all(x() is not None for x in old) and ws._o_acc is not old[0]()
+    # growing one row at a time: what is held stays within a small multiple of what is needed
+    for rows in range(1, 400):
+        o, lse = ws.partials(1, 4, 8, rows, 64, device)
+        assert o.shape == (1, 4, 8, rows, 64) and lse.shape == (1, 4, 8, rows)
+    held = sum(x.numel() for x in [ws._o_acc, ws._lse_acc, *ws._outgrown])
+    assert held <= 5 * (o.numel() + lse.numel())
