@@ -148,7 +148,8 @@ class PagedAttention(torch.nn.Module):
     def evict(self, k_cache, v_cache, weights, seqlen_k, block_table, new_block_table, *, budget: int, recent: int = 0, sinks: int = 0,
               **outputs):
         """Keep the `budget` keys of every (sequence, KV head) that received the most weight and move them to new pages; see
-        `fmha_cache_evict`.  Not with a sliding window: evicted keys have no positions.
+        `fmha_cache_evict`.  Not with a sliding window: evicted keys have no positions.  `decode_step` rotates by the cached count, which
+        an eviction makes smaller than the position: `fmha_cache_evict` says what to pass instead.
         Returns (seqlen_k_new, kept, weights_new)."""
         if self.window_left >= 0:
             raise ValueError("a cache read through a sliding window cannot be evicted from: its keys lose their positions")

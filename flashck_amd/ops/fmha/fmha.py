@@ -1159,7 +1159,9 @@ def fmha_cache_evict(k_cache, v_cache, weights, seqlen_k, block_table, new_block
     [B, pages], at least `budget` keys a row) receives, for each head, the row of its j-th kept key in ascending order.
     The rows go to new_k_cache / new_v_cache (default: the same pools); pages that block_table names are never written, as other
     sequences may share them, so new_block_table must name other pages then.  After the call the old pages can be reused.
-    Heads keep different positions: masks that go by position do not apply to evicted keys any more.
+    Heads keep different positions: masks that go by position do not apply to evicted keys any more, and an append that rotates
+    (fmha_decode_step with rotary tables) takes a sequence's new, smaller key count for its position: rotate the new tokens at
+    their true positions before, or pass tables whose first row is the number of keys evicted (the same for every sequence).
 
     Returns (seqlen_k_new int32 [B], kept int32 [B, Hk, budget] with -1 behind the n-th, weights_new fp32 [B, Hk, cols] with
     zeros behind the n-th)."""
