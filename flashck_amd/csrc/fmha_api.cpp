@@ -601,6 +601,8 @@ int fck_fmha_fwd_splitkv_combine_lse(const void* lse_acc, const void* o_acc, voi
     a.num_splits = (int32_t)num_splits;
     a.num_cu = cu_count();
     a.lse = static_cast<float*>(lse);
+    a.seqstart_q = seqstart_q;
+    a.batch = (int32_t)batch;
     a.o_scale = 1.f;  // e4m3 output: the reference's wrapper has no scale argument either (fmha_fwd_split_kv_combine_jinja.h:78-92)
     return launch_status(fck::launch_splitkv_combine(a, dtype, static_cast<hipStream_t>(stream)), "FmhaFwdSplitKVCombine launch");
 }

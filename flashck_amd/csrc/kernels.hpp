@@ -64,6 +64,8 @@ struct CombineArgs {
     int32_t num_cu;  // compute units of the device (decides the workgroup size)
     float o_scale;   // e4m3 output: O = saturate(o_scale * o)
     float* lse;      // [Bs, Hq, Sq] log-sum-exp of every row, or null
+    const int32_t* seqstart_q;  // packed queries: rows at and behind seqstart_q[batch] have no partial results
+    int32_t batch;
 };
 
 struct AppendKvArgs {

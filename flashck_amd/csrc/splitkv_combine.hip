@@ -27,6 +27,7 @@ __global__ __launch_bounds__(NT) void splitkv_combine_kernel(const CombineArgs a
     const int64_t row = item / a.hq;  // b * Sq + i
     const int h = (int)(item % a.hq);
     const int64_t b = row / a.Sq, i = row % a.Sq;
+    if (a.seqstart_q && row >= a.seqstart_q[a.batch]) return;  // a row behind the last sequence stays as it was
     const int ns = a.num_splits;
     const int64_t w0 = ((b * a.hq + h) * ns) * a.Sq + i;  // split 0; next split is Sq further
 

@@ -244,3 +244,21 @@ def test_a_captured_call_survives_a_workspace_that_grows(fmha):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and all((x == 7.0).all() for x in others)
+
+
+@pytest.mark.parametrize("splits", [1, 3])
+def test_rows_behind_the_last_sequence_stay_as_they_were(fmha, splits):
+    lens, starts = [90, 40], [0, 3, 4]
+    g = torch.Generator().manual_seed(12)
+    kc, vc, table = lc.pages(g, lens, 16, 2, 64, 64, torch.bfloat16)
+    q = lc.randn(g, 9, 4, 64, dtype=torch.bfloat16)   # five rows behind the last sequence
+    kw = dict(mask_type=2, window=(-1, 0))
+    ref, ref_lse = lc.decode(q, kc, vc, lens, table, 0.125, starts=starts, **kw)
+    out, lse = dev(torch.full((9, 4, 64), 3.0, dtype=torch.bfloat16)), dev(torch.full((4, 9), 7.0))
+    ws = (dev(torch.full((1, 4, splits, 9, 64), 5.0)), dev(torch.full((1, 4, splits, 9), 5.0)))
+    fmha.fmha_decode_paged(dev(q), dev(kc), dev(vc), _i32(lens), dev(table), num_splits=splits, cu_seqlens_q=_i32(starts), max_seqlen_q=3,
+                           workspace=ws, out=out, lse=lse, **kw)
+    out, lse = out.cpu(), lse.cpu()
+    assert (out[:4].double() - ref[:4]).abs().max() <= (2 * U[torch.bfloat16] + 2.0 ** -20) * 6.0
+    assert (lse[:, :4].double() - ref_lse[:, :4]).abs().max() <= 2e-5
+    assert (out[4:] == 3.0).all() and (lse[:, 4:] == 7.0).all()
