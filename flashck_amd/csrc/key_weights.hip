@@ -65,6 +65,47 @@ struct StepShape {
     static constexpr int KT = D / 32;
 };
 
+// requests the 32 keys from kb on, whose rows hold row_bytes of S::ROWB, into the calling wave's tile
+template <typename S>
+__device__ __forceinline__ void request_keys(const KeyWeightsArgs& a, const KvSeq& ks, bool uniform, int sk, int hkv, int row_bytes,
+                                             char FCK_LDS* tile, int kb)
+{
+    const int lane = threadIdx.x & 63;
+    int64_t row0 = ks.base_row + kb;
+    if (uniform && ks.table) {
+        const int pi = a.kv.page_shift >= 0 ? kb >> a.kv.page_shift : kb / a.kv.page_size;
+        row0 = (int64_t)const_load(ks.table, pi) * a.kv.page_size + (kb - pi * a.kv.page_size);
+    }
+#pragma unroll
+    for (int u = 0; u < S::LD; ++u) {
+        const int off = u * 1024 + lane * 16;
+        const int row = off / S::ROWB;
+        const int chunk = (off % S::ROWB / 16) ^ chunk_swizzle<S::CH>(row);
+        const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_address(tile + u * 1024));
+        if (chunk * 16 >= row_bytes) {  // the stored row is shorter than D: these places were zeroed once
+            FCK_LOAD_TO_LDS_MASKED();
+            continue;
+        }
+        const int in = min(row, sk - 1 - kb);  // rows past the last key repeat it, and are not stored
+        const int64_t cr = uniform ? row0 + in : kv_row(a.kv, ks, kb + in);
+        load_to_lds_stream(dst, (const char*)a.k + (cr * a.hk + hkv) * row_bytes + chunk * 16);
+    }
+}
+
+// zeroes the places of a tile that no request fills
+template <typename S>
+__device__ __forceinline__ void clear_missing(char FCK_LDS* tile, int row_bytes)
+{
+    if (row_bytes >= S::ROWB) return;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int u = 0; u < S::LD; ++u) {
+        const int off = u * 1024 + lane * 16;
+        const int row = off / S::ROWB;
+        if (((off % S::ROWB / 16) ^ chunk_swizzle<S::CH>(row)) * 16 >= row_bytes) *(u32x4_t FCK_LDS*)(tile + off) = u32x4_t{0u, 0u, 0u, 0u};
+    }
+}
+
 template <typename T, int D, int MB, int NT, bool kMod, bool kKv8>
 __global__ __launch_bounds__(256) void key_weights_step_kernel(const KeyWeightsArgs a)
 {
@@ -93,38 +134,9 @@ __global__ __launch_bounds__(256) void key_weights_step_kernel(const KeyWeightsA
     const int n = key0 < key1 ? (int)min((int64_t)NT, (key1 - key0 + 31) / 32) : 0;
 
     const bool uniform = ks.table == nullptr || a.kv.page_size % 32 == 0;  // a tile never straddles a page
-    const char* const kp = (const char*)a.k;
     const int row_bytes = a.d * (kKv8 ? 1 : 2);
-    auto request = [&](int c) __attribute__((always_inline)) {
-        const int kb = (int)key0 + c * 32;
-        int64_t row0 = ks.base_row + kb;
-        if (uniform && ks.table) {
-            const int pi = a.kv.page_shift >= 0 ? kb >> a.kv.page_shift : kb / a.kv.page_size;
-            row0 = (int64_t)const_load(ks.table, pi) * a.kv.page_size + (kb - pi * a.kv.page_size);
-        }
-#pragma unroll
-        for (int u = 0; u < S::LD; ++u) {
-            const int off = u * 1024 + lane * 16;
-            const int row = off / S::ROWB;
-            const int chunk = (off % S::ROWB / 16) ^ chunk_swizzle<S::CH>(row);
-            const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_address(tiles + u * 1024));
-            if (chunk * 16 >= row_bytes) {  // the stored row is shorter than D: these places were zeroed once
-                FCK_LOAD_TO_LDS_MASKED();
-                continue;
-            }
-            const int in = min(row, sk - 1 - kb);  // rows past the last key repeat it, and are not stored
-            const int64_t cr = uniform ? row0 + in : kv_row(a.kv, ks, kb + in);
-            load_to_lds_stream(dst, kp + (cr * a.hk + hkv) * row_bytes + chunk * 16);
-        }
-    };
-    if (row_bytes < S::ROWB) {
-#pragma unroll
-        for (int u = 0; u < S::LD; ++u) {
-            const int off = u * 1024 + lane * 16;
-            const int row = off / S::ROWB;
-            if (((off % S::ROWB / 16) ^ chunk_swizzle<S::CH>(row)) * 16 >= row_bytes) *(u32x4_t FCK_LDS*)(tiles + off) = u32x4_t{0u, 0u, 0u, 0u};
-        }
-    }
+    auto request = [&](int c) __attribute__((always_inline)) { request_keys<S>(a, ks, uniform, sk, hkv, row_bytes, tiles, (int)key0 + c * 32); };
+    clear_missing<S>(tiles, row_bytes);
     if (n > 0) request(0);
 
     const int tok0 = __builtin_amdgcn_readfirstlane(a.seqstart_q ? a.seqstart_q[b] : b * a.sq);
@@ -338,36 +350,8 @@ __global__ __launch_bounds__(512) void key_weights_window_kernel(const KeyWeight
     const int q_bytes = a.d * 2, k_bytes = a.d * (kKv8 ? 1 : 2);
 
     const bool uniform = ks.table == nullptr || a.kv.page_size % 32 == 0;  // a tile never straddles a page
-    auto request = [&](int c) __attribute__((always_inline)) {
-        const int kb = (int)key0 + c * 32;
-        int64_t row0 = ks.base_row + kb;
-        if (uniform && ks.table) {
-            const int pi = a.kv.page_shift >= 0 ? kb >> a.kv.page_shift : kb / a.kv.page_size;
-            row0 = (int64_t)const_load(ks.table, pi) * a.kv.page_size + (kb - pi * a.kv.page_size);
-        }
-#pragma unroll
-        for (int u = 0; u < S::LD; ++u) {
-            const int off = u * 1024 + lane * 16;
-            const int row = off / S::ROWB;
-            const int chunk = (off % S::ROWB / 16) ^ chunk_swizzle<S::CH>(row);
-            const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_address(tile + u * 1024));
-            if (chunk * 16 >= k_bytes) {  // the stored row is shorter than D: these places were zeroed once
-                FCK_LOAD_TO_LDS_MASKED();
-                continue;
-            }
-            const int in = min(row, sk - 1 - kb);  // rows past the last key repeat it, and are not stored
-            const int64_t cr = uniform ? row0 + in : kv_row(a.kv, ks, kb + in);
-            load_to_lds_stream(dst, (const char*)a.k + (cr * a.hk + hkv) * k_bytes + chunk * 16);
-        }
-    };
-    if (k_bytes < S::ROWB) {
-#pragma unroll
-        for (int u = 0; u < S::LD; ++u) {
-            const int off = u * 1024 + lane * 16;
-            const int row = off / S::ROWB;
-            if (((off % S::ROWB / 16) ^ chunk_swizzle<S::CH>(row)) * 16 >= k_bytes) *(u32x4_t FCK_LDS*)(tile + off) = u32x4_t{0u, 0u, 0u, 0u};
-        }
-    }
+    auto request = [&](int c) __attribute__((always_inline)) { request_keys<S>(a, ks, uniform, sk, hkv, k_bytes, tile, (int)key0 + c * 32); };
+    clear_missing<S>(tile, k_bytes);
     if (n > 0) request(0);
 #pragma unroll
     for (int j = 0; j < S::NT / 2; ++j) {
