@@ -262,3 +262,59 @@ def test_rows_behind_the_last_sequence_stay_as_they_were(fmha, splits):
     assert (out[:4].double() - ref[:4]).abs().max() <= (2 * U[torch.bfloat16] + 2.0 ** -20) * 6.0
     assert (lse[:, :4].double() - ref_lse[:, :4]).abs().max() <= 2e-5
     assert (out[4:] == 3.0).all() and (lse[:, 4:] == 7.0).all()
+
+
+@pytest.mark.parametrize("window_left", [-1, 40])
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_module_steps_over_shared_prefixes(fmha, window_left, packed, fp8):
+    """PagedAttention: three steps with prefix_lens and without on caches of their own, the weights of the last step's keys, and an
+    eviction: what a serving loop runs.  Bounds of the outputs: both sides within 2 u max|v| of the definition, max|v| < 6."""
+    from flashck_amd.nn import PagedAttention
+    g = torch.Generator().manual_seed(13)
+    lens, page, hq, hk, d = [100, 90, 130, 40, 33], 16, 8, 2, 64
+    starts, prefixes, counts = [0, 3, 5], [70, 20], ([2, 1, 0, 3, 2] if packed else [2] * 5)
+    kc, vc, table = lc.pages(g, [n + 10 for n in lens], page, hk, d, d, torch.bfloat16, fp8, extra=20, poison=False)
+    lc.share(kc, vc, table, starts, prefixes, page)
+    kd, vd = (0.5, 0.25) if fp8 else (1.0, 1.0)
+    modules = [PagedAttention(hq, hk, d, window_left=window_left, rope_mode=fmha.ROPE_HALF_ROTATED, k_descale=kd, v_descale=vd) for _ in range(2)]
+    caches = [(dev(kc.clone()), dev(vc.clone())) for _ in range(2)]
+    angles = torch.arange(200)[:, None] * torch.exp(-torch.arange(0, d, 2) / d * 9.0)
+    rotary = dict(rotary_cos=dev(torch.cos(angles).to(torch.bfloat16)), rotary_sin=dev(torch.sin(angles).to(torch.bfloat16)))
+    cu = [0]
+    for n in counts:
+        cu.append(cu[-1] + n)
+    extra = dict(cu_seqlens_knew=_i32(cu), max_seqlen_knew=3) if packed else {}
+    shape, total = ((cu[-1],) if packed else (5, 2)), cu[-1]
+    now = [_i32(lens), _i32(lens)]
+    dt = dev(table)
+    for step in range(3):
+        q, kn, vn = (lc.randn(g, *shape, h, d, dtype=torch.bfloat16) for h in (hq, hk, hk))
+        lse = [dev(torch.zeros(*((hq, total) if packed else (5, hq, 2)))) for _ in range(2)]
+        outs, queries = [], []
+        for k, m in enumerate(modules):
+            queries.append(dev(q.clone()))
+            prefix = dict(prefix_lens=_i32(prefixes), cu_groups=_i32(starts)) if k == 0 else {}
+            o, n = m.decode_step(queries[k], dev(kn), dev(vn), *caches[k], now[k], dt, lse=lse[k], **rotary, **extra, **prefix)
+            outs.append(o.cpu())
+            now[k] = n.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(now[0].cpu(), now[1].cpu())
+        for a, b in zip(*caches):
+            assert torch.equal(a.cpu().view(torch.uint8), b.cpu().view(torch.uint8))
+        assert torch.equal(queries[0].cpu(), queries[1].cpu())   # rotated in place
+        assert torch.isfinite(outs[0].float()).all()
+        assert (outs[0].double() - outs[1].double()).abs().max() <= 4 * U[torch.bfloat16] * 6.0
+        assert (lse[0].cpu() - lse[1].cpu()).abs().max() <= 4e-5
+    assert now[0].cpu().tolist() == [n + 3 * c for n, c in zip(lens, counts)]
+    more = dict(cu_seqlens_q=_i32(cu), max_seqlen_q=3) if packed else {}
+    w = modules[0].key_weights(queries[0], caches[0][0], lse[0], now[0], dt, **more)
+    # every row gives its heads a weight of one each
+    rows = torch.tensor(counts, dtype=torch.float64)[:, None] * (hq // hk)
+    assert (w.cpu().double().sum(dim=2) - rows).abs().max() <= 1e-4 * rows.max()
+    if window_left >= 0:
+        return
+    free = sorted(set(range(kc.shape[0])) - set(table.flatten().tolist()))[:10]
+    n_new, kept, _ = modules[0].evict(*caches[0], w, now[0], dt, _i32(free).view(5, 2), budget=32, recent=4)
+    torch.cuda.synchronize()
+    assert kept.cpu().tolist() == lc.evict(w.cpu(), now[0].cpu().tolist(), 32, 4, 0) and n_new.cpu().tolist() == [32] * 5
