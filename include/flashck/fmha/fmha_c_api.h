@@ -323,7 +323,8 @@ FCK_EXPORT int fck_fmha_shared_prefix_splits(int64_t batch, int64_t num_groups, 
  *   out[b, hk, t] = weights[b, hk, t] + sum over the query heads h of KV head hk and the rows i that see key t of
  *                   exp(s - lse[b, h, i]),  s the score of (b, h, i, t) as the attention entry points define it
  *   lse      fp32 [B, Hq, sq] (group mode [Hq, total_q]): the log-sum-exp the attention over the same keys returned
- *            (fck_fmha_attrs.lse, _combine_lse, fck_fmha_decode_shared_prefix); a row with -inf adds nothing
+ *            (fck_fmha_attrs.lse, _combine_lse, fck_fmha_decode_shared_prefix); a row with -inf adds nothing, whatever its
+ *            queries hold
  *   weights, out  fp32 [B, Hk, cols]; weights may be NULL (zeros) or out itself.  Entries at and behind a sequence's key
  *            count are written as 0; keys at and behind cols have no entry.
  *   workspace  fp32 [num_row_splits, B, Hk, cols] when num_row_splits > 1 (in [1, 16]; fck_fmha_key_weights_row_splits chooses:
@@ -357,7 +358,8 @@ FCK_EXPORT int fck_fmha_key_weights_row_splits(int64_t batch, int64_t q_num_head
  *   workspace     device memory of fck_fmha_cache_evict_workspace_bytes bytes (16-byte aligned; what it holds does not matter), or
  *                 NULL: with it the choice among few long rows is spread over the chip
  * dtype is the element type of the caches.  The positions of a head's kept keys differ between heads, so masks that go by
- * position do not apply to the evicted keys.  No counterpart in the reference.
+ * position do not apply to the evicted keys.  A budget or a block-table row beyond 2^30 keys, and a move of more than 2^31 8- or
+ * 16-byte pieces per 4 slots, are refused before anything is written.  No counterpart in the reference.
  */
 FCK_EXPORT int fck_fmha_cache_evict(const void* k_cache, const void* v_cache, void* new_k_cache, void* new_v_cache,
                                     const void* weights, void* new_weights, void* workspace, const int32_t* seqlen_k,
