@@ -978,6 +978,8 @@ int fck_fmha_decode_shared_prefix(const void* q, const void* k_cache, const void
     if (seqlen_q <= 0) return fail(FCK_ERR_INVALID_ARGUMENT, "seqlen_q must be positive (group mode: it carries total_q)");
     if (q_max_seq_len <= 0 || q_max_seq_len > seqlen_q) q_max_seq_len = seqlen_q;
     if (num_groups < 1 || (!cu_groups && num_groups != 1)) return fail(FCK_ERR_INVALID_ARGUMENT, "num_groups must be positive, and 1 without cu_groups");
+    // sequences of a group as a rule: what the caller says, else the average
+    const int64_t typical = max_group_size > 0 && max_group_size < batch ? max_group_size : (batch - 1) / num_groups + 1;
     if (max_group_size <= 0 || max_group_size > batch) max_group_size = batch;
     if (num_prefix_splits < 1 || num_prefix_splits > 64 || num_own_splits < 1 || num_own_splits > 64)
         return fail(FCK_ERR_INVALID_ARGUMENT, "num_prefix_splits %ld / num_own_splits %ld out of range [1,64]", (long)num_prefix_splits, (long)num_own_splits);
@@ -987,8 +989,9 @@ int fck_fmha_decode_shared_prefix(const void* q, const void* k_cache, const void
     int64_t tokens = max_group_size * q_max_seq_len;
     if (seqstart_q && tokens > seqlen_q) tokens = seqlen_q;
     const int64_t g = hq / hk;
+    const int64_t all = (seqstart_q ? 1 : batch) * seqlen_q;
     if (int rc = check_fit32(tokens)) return rc;
-    if (int rc = check_fit32(q_max_seq_len * g, tokens * g, batch * hk, num_groups * hk)) return rc;
+    if (int rc = check_fit32(q_max_seq_len * g, tokens * g, all * g, batch * hk, num_groups * hk)) return rc;
     // Fewest keys per split: the equal parts of the bound, but never more than `most`, which is what a loose bound comes to.
     // 32 sequences on 4096 shared keys, bounds of 131072: 31 us with 256 for the prefix, 34 us with 128; 4 sequences on 512 shared
     // keys, bounds of 32768: 17.5 and 15 us.  Own keys, exact bounds, the first batch: 25.2 us with 256, 25.8 us with 128.
@@ -1038,7 +1041,8 @@ int fck_fmha_decode_shared_prefix(const void* q, const void* k_cache, const void
     if (int rc = only_score_attrs(attrs)) return rc;
     if (int rc = fill_cache_type(a.kv8, a.scale_log2, a.mod, &a.v_descale, attrs, d, dv)) return rc;
     g_kernel = "shared_prefix_kernel";
-    return launch_status(fck::launch_shared_prefix(a, kernel_dim(d, dv), dtype, tokens * g, q_max_seq_len * g,
+    const int64_t rule = typical * q_max_seq_len < tokens ? typical * q_max_seq_len : tokens;
+    return launch_status(fck::launch_shared_prefix(a, kernel_dim(d, dv), dtype, {tokens * g, rule * g, q_max_seq_len * g, all * g},
                                                    static_cast<hipStream_t>(stream)), "shared-prefix decode launch");
 }
 

@@ -131,7 +131,8 @@ struct SharedPrefixArgs {
     int32_t sq, hq, hk, d, dv;
     int32_t ns_prefix, ns_own;
     int32_t prefix_chunk, own_chunk;  // fewest keys per split (multiples of 64)
-    int32_t prefix_tiles, own_tiles;  // row tiles per (group, KV head) / per (sequence, KV head); set by the launcher
+    int32_t prefix_tiles;             // row tiles per (group, KV head); 0: the tiles of all groups are numbered in one row; set by the launcher
+    int32_t own_tiles;                // row tiles per (sequence, KV head); set by the launcher
     int32_t prefix_items;             // workgroups that handle prefixes; set by the launcher
     int64_t shape_sq;                 // Sq of the workspace: sq (batch mode) or total_q
     float scale_log2;
@@ -144,8 +145,11 @@ struct SharedPrefixArgs {
 };
 // 16-row blocks per wave for groups of rows_prefix packed rows
 int shared_prefix_blocks(int d, int64_t rows_prefix);
-// rows_prefix / rows_own: most packed query rows of a group / of a sequence
-hipError_t launch_shared_prefix(SharedPrefixArgs a, int d, int dtype, int64_t rows_prefix, int64_t rows_own, hipStream_t st);
+// packed query rows: of a group at most, of a group as a rule, of a sequence at most, of the batch; each below 2^31
+struct SharedPrefixRows {
+    int64_t group, typical, own, all;
+};
+hipError_t launch_shared_prefix(SharedPrefixArgs a, int d, int dtype, const SharedPrefixRows& rows, hipStream_t st);
 
 // Attention weight every key of a cache receives (key_weights.hip).
 struct KeyWeightsArgs {

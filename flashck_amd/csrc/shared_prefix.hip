@@ -13,7 +13,9 @@
 //   [lo, hi) of its own (its sequence's length and mask decide), so an item never has to know where its rows come from
 //   after it has set them up.
 //   Prefix items come first (they are the long ones); those that stream the same keys get ids congruent modulo 8, i.e. one
-//   XCD and one L2.
+//   XCD and one L2.  Groups take equally many row tiles each when the caller bounds their size; otherwise the tiles of all
+//   groups are numbered in one row, tile floor(first row / BM) + g being the first of group g: ceil(x - y) <= floor(x) -
+//   floor(y) + 1, so every group has the tiles it needs, and there is one idle tile per group at most.
 //   Every slot of every row is written (an empty one as lse = -inf), so the merge reads no lengths and no groups.
 //
 // What bounds it: a small group reads its keys (32 sequences on 4096 shared and up to 1024 own keys, 8 KV heads of 4 query
@@ -68,6 +70,29 @@ __device__ __forceinline__ int own_begin(const SharedPrefixArgs& a, int b)
     return b >= s.first && b < s.first + s.count ? s.prefix : 0;
 }
 
+// first row tile of group i when the tiles of all groups are numbered in one row; g packed rows per query token
+template <int BM>
+__device__ __forceinline__ int first_tile(const SharedPrefixArgs& a, int i, int g)
+{
+    const int b = a.cu_groups ? min(max(a.cu_groups[i], 0), a.batch) : 0;
+    return (a.seqstart_q ? a.seqstart_q[b] : b * a.sq) * g / BM + i;
+}
+
+// the last group whose first tile is at or before t
+template <int BM>
+__device__ __forceinline__ int group_of_tile(const SharedPrefixArgs& a, int t, int g)
+{
+    int lo = 0, hi = a.groups - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (first_tile<BM>(a, mid, g) <= t)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    return lo;
+}
+
 template <int D, int MB>
 struct SharedShape {
     static constexpr int TK = D == 256 ? 32 : 64;  // keys per tile
@@ -120,10 +145,18 @@ __global__ __launch_bounds__(256, (kSharedWaves<D, MB>)) void shared_prefix_kern
     int hkv, split, ns, slot, mt, leader, key_lo, key_hi, tok0, tok1;
     if (prefix) {
         constexpr int kXcd = 8;
-        const int s = id / kXcd;
-        mt = s % a.prefix_tiles;
-        const int stream = s / a.prefix_tiles * kXcd + id % kXcd;
-        if (stream >= a.groups * a.ns_prefix * a.hk) return;
+        const int s = id / kXcd, per = max(a.prefix_tiles, 1);
+        mt = s % per;
+        int stream = s / per * kXcd + id % kXcd;
+        if (a.prefix_tiles > 0) {
+            if (stream >= a.groups * a.ns_prefix * a.hk) return;
+        } else {
+            const int combos = a.ns_prefix * a.hk;
+            const int group = group_of_tile<S::BM>(a, id / combos, g);
+            mt = id / combos - first_tile<S::BM>(a, group, g);
+            if (mt < 0) return;  // rows of sequences before the first group
+            stream = group * combos + id % combos;
+        }
         hkv = stream % a.hk;
         split = slot = stream / a.hk % a.ns_prefix;
         ns = a.ns_prefix;
@@ -460,15 +493,19 @@ hipError_t launch_combine(const SharedPrefixArgs& a, hipStream_t st)
 }
 
 template <typename T, int D, int MB>
-hipError_t launch_mb(SharedPrefixArgs& a, int64_t rows_prefix, int64_t rows_own, hipStream_t st)
+hipError_t launch_mb(SharedPrefixArgs& a, const SharedPrefixRows& rows, hipStream_t st)
 {
     constexpr int BM = SharedShape<D, MB>::BM;
-    const int64_t p_tiles = (rows_prefix + BM - 1) / BM, o_tiles = (rows_own + BM - 1) / BM;
+    const int64_t p_tiles = (rows.group + BM - 1) / BM, o_tiles = (rows.own + BM - 1) / BM;
     const int64_t streams = ((int64_t)a.groups * a.ns_prefix * a.hk + 7) / 8 * 8;
-    const int64_t prefix_items = streams * p_tiles;
+    // Equally many tiles per group, unless the bound on their size makes that more than twice what all rows can need (256
+    // sequences in 64 groups without a bound: 213 us so, 94 us with the tiles in one row, 92 us with an exact bound).
+    const int64_t all_tiles = rows.all / BM + a.groups;
+    const bool equal = p_tiles * a.groups <= 2 * all_tiles;
+    const int64_t prefix_items = equal ? streams * p_tiles : (int64_t)a.ns_prefix * a.hk * all_tiles;
     const int64_t grid = prefix_items + (int64_t)a.hk * a.ns_own * o_tiles * a.batch;
-    if (p_tiles > INT32_MAX || o_tiles > INT32_MAX || grid > INT32_MAX) return hipErrorInvalidValue;
-    a.prefix_tiles = (int32_t)p_tiles;
+    if (grid > INT32_MAX) return hipErrorInvalidValue;
+    a.prefix_tiles = equal ? (int32_t)p_tiles : 0;
     a.own_tiles = (int32_t)o_tiles;
     a.prefix_items = (int32_t)prefix_items;
     // a key tile then never straddles a page
@@ -480,11 +517,11 @@ hipError_t launch_mb(SharedPrefixArgs& a, int64_t rows_prefix, int64_t rows_own,
 }
 
 template <typename T, int D>
-hipError_t launch_d(SharedPrefixArgs& a, int64_t rows_prefix, int64_t rows_own, hipStream_t st)
+hipError_t launch_d(SharedPrefixArgs& a, const SharedPrefixRows& rows, hipStream_t st)
 {
     if constexpr (D <= 128)
-        if (shared_prefix_blocks(D, rows_prefix) == 2) return launch_mb<T, D, 2>(a, rows_prefix, rows_own, st);
-    return launch_mb<T, D, 1>(a, rows_prefix, rows_own, st);
+        if (shared_prefix_blocks(D, rows.typical) == 2) return launch_mb<T, D, 2>(a, rows, st);
+    return launch_mb<T, D, 1>(a, rows, st);
 }
 
 }  // namespace
@@ -493,12 +530,12 @@ hipError_t launch_d(SharedPrefixArgs& a, int64_t rows_prefix, int64_t rows_own, 
 // (half as many items then share out the keys).
 int shared_prefix_blocks(int d, int64_t rows_prefix) { return d <= 128 && rows_prefix > 128 ? 2 : 1; }
 
-hipError_t launch_shared_prefix(SharedPrefixArgs a, int d, int dtype, int64_t rows_prefix, int64_t rows_own, hipStream_t st)
+hipError_t launch_shared_prefix(SharedPrefixArgs a, int d, int dtype, const SharedPrefixRows& rows, hipStream_t st)
 {
     switch (d) {
-    case 64: return dtype == 4 ? launch_d<BF16, 64>(a, rows_prefix, rows_own, st) : launch_d<FP16, 64>(a, rows_prefix, rows_own, st);
-    case 128: return dtype == 4 ? launch_d<BF16, 128>(a, rows_prefix, rows_own, st) : launch_d<FP16, 128>(a, rows_prefix, rows_own, st);
-    case 256: return dtype == 4 ? launch_d<BF16, 256>(a, rows_prefix, rows_own, st) : launch_d<FP16, 256>(a, rows_prefix, rows_own, st);
+    case 64: return dtype == 4 ? launch_d<BF16, 64>(a, rows, st) : launch_d<FP16, 64>(a, rows, st);
+    case 128: return dtype == 4 ? launch_d<BF16, 128>(a, rows, st) : launch_d<FP16, 128>(a, rows, st);
+    case 256: return dtype == 4 ? launch_d<BF16, 256>(a, rows, st) : launch_d<FP16, 256>(a, rows, st);
     }
     return hipErrorInvalidValue;
 }

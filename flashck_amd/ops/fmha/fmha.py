@@ -1049,13 +1049,15 @@ def fmha_decode_shared_prefix(q, k_cache, v_cache, seqlen_k, block_table, prefix
     capacity = block_table.shape[1] * page
     if capacity == 0:
         raise ValueError("block_table must have at least one page per sequence")
-    max_group_size = min(int(max_group_size), B) if max_group_size > 0 else B
+    # sequences of a group: at most (0: any number), and as a rule
+    max_group_size = int(max_group_size) if 0 < max_group_size < B else 0
+    typical = max_group_size or -(-B // G)
     # the longest prefix, and the keys a sequence that has it has behind it; they steer the splits and nothing else
     longest = min(max_seqlen_k, capacity) if max_seqlen_k > 0 else capacity
     prefix = min(max_prefix_len, longest) if max_prefix_len > 0 else longest
     own = max(longest - prefix, 1)
     if num_prefix_splits <= 0 or num_splits <= 0:
-        ns = _shared_prefix_splits(q.device, B, G, max_group_size, Hq, Hk, sq_max, max(D, Dv), prefix, own, longest)
+        ns = _shared_prefix_splits(q.device, B, G, typical, Hq, Hk, sq_max, max(D, Dv), prefix, own, longest)
         num_prefix_splits = num_prefix_splits if num_prefix_splits > 0 else ns[0]
         num_splits = num_splits if num_splits > 0 else ns[1]
     if flags.flag("FC_DEBUG_KERNEL_INSTANCE"):

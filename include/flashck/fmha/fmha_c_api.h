@@ -288,7 +288,7 @@ FCK_EXPORT int fck_fmha_fwd_splitkv_combine_lse(const void* lse_acc, const void*
  *   prefix_lens   int32 [num_groups]: tokens the group's sequences have in common, from their first on (any count; clamped
  *                 to what the group's first sequence has).  They are read through the first sequence's block-table row, so
  *                 the rows of the others need not be set up for whole pages of them.
- *   max_group_size  at most this many sequences of a group share (0: batch); the ones behind read all their own keys
+ *   max_group_size  at most this many sequences of a group share (0: any number); the ones behind read all their own keys
  *   seqlen_k_ptr  int32 [B], key counts with the prefix
  *   q, o, lse     as fck_fmha_fwd_splitkv and its combine; seqlen_q carries total_q in group mode; lse may be NULL
  *   max_prefix_len, max_own_len  the longest prefix and the most keys a sequence has behind it (0: what the table can address).

@@ -318,3 +318,39 @@ def test_module_steps_over_shared_prefixes(fmha, window_left, packed, fp8):
     n_new, kept, _ = modules[0].evict(*caches[0], w, now[0], dt, _i32(free).view(5, 2), budget=32, recent=4)
     torch.cuda.synchronize()
     assert kept.cpu().tolist() == lc.evict(w.cpu(), now[0].cpu().tolist(), 32, 4, 0) and n_new.cpu().tolist() == [32] * 5
+
+
+# (sizes of the groups, sequences before the first and behind the last, tokens a sequence, query heads of the 1 KV head, head dim)
+MANY_GROUPS = [([2] * 10, 0, 0, 1, 16, 64), ([1, 9, 1, 1, 0, 3, 1, 1, 1, 2], 3, 2, 1, 16, 64), ([1] * 12, 5, 0, 2, 8, 128), ([2, 2, 3, 2], 1, 1, 5, 16, 64),
+               ([3, 1, 2, 2, 2], 0, 0, 4, 12, 256)]
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("sizes,before,behind,sq,hq,d", MANY_GROUPS)
+def test_many_groups_without_a_bound_on_their_size(fmha, sizes, before, behind, sq, hq, d, packed):
+    # so many that the row tiles are not dealt out equally: groups of one tile, of several, empty ones, rows of no group; sequences share
+    # whole pages only (page 16, prefixes of 0, 16, 32)
+    g = torch.Generator().manual_seed(14)
+    starts = [before]
+    for s in sizes:
+        starts.append(starts[-1] + s)
+    batch = starts[-1] + behind
+    prefixes = [(0, 32, 16, 32)[k % 4] for k in range(len(sizes))]
+    lens = [35 + b % 5 * 9 for b in range(batch)]
+    kc, vc, table = lc.pages(g, lens, 16, 1, d, d, torch.bfloat16)
+    lc.share(kc, vc, table, starts, prefixes, 16)
+    counts = [(sq, 0, 1, sq)[b % 4] for b in range(batch)] if packed else [sq] * batch
+    cu = [0]
+    for n in counts:
+        cu.append(cu[-1] + n)
+    q = lc.randn(g, *((cu[-1],) if packed else (batch, sq)), hq, d, dtype=torch.bfloat16)
+    kw = dict(mask_type=2, window=(-1, 0))
+    ref, ref_lse = lc.decode(q, kc, vc, lens, table, d ** -0.5, starts=cu if packed else None, **kw)
+    lse = dev(torch.zeros(ref_lse.shape))
+    if packed:
+        kw.update(cu_seqlens_q=_i32(cu), max_seqlen_q=sq)
+    for nsp in (1, 3):
+        o = fmha.fmha_decode_shared_prefix(dev(q), dev(kc), dev(vc), _i32(lens), dev(table), _i32(prefixes), cu_groups=_i32(starts), lse=lse,
+                                           num_prefix_splits=nsp, num_splits=2, **kw).cpu()
+        assert (o.double() - ref).abs().max() <= (2 * U[torch.bfloat16] + 2.0 ** -20) * 6.0
+        assert (lse.cpu().double() - ref_lse).abs().max() <= 2e-5

@@ -123,3 +123,17 @@ def test_an_outgrown_workspace_buffer_stays_allocated():
         assert o.shape == (1, 4, 8, rows, 64) and lse.shape == (1, 4, 8, rows)
     held = sum(x.numel() for x in [ws._o_acc, ws._lse_acc, *ws._outgrown])
     assert held <= 5 * (o.numel() + lse.numel())
+
+
+def test_a_missing_bound_on_the_groups_takes_them_for_average(monkeypatch):
+    seen, call = [], F._call
+    monkeypatch.setattr(F, "_REQUIRE_GPU_TENSORS", False)
+    monkeypatch.setattr(F, "_stream", lambda: None)
+    monkeypatch.setattr(F, "_call", lambda name, *args: seen.append(args) if name == "fck_fmha_decode_shared_prefix" else call(name, *args))
+    cache = torch.zeros(1, 64, 8, 128, dtype=torch.bfloat16)
+    cu, lens = torch.arange(65, dtype=torch.int32) * 4, torch.full((256,), 1100, dtype=torch.int32)
+    for bound in (0, 4, 256, 1000):
+        F.fmha_decode_shared_prefix(torch.zeros(256, 1, 32, 128, dtype=torch.bfloat16), cache, cache, lens, torch.zeros(256, 20, dtype=torch.int32),
+                                    torch.full((64,), 1024, dtype=torch.int32), cu_groups=cu, max_group_size=bound)
+    # no bound, the exact one, and bounds that say nothing: the same splits; the library is told of the exact one only
+    assert len({a[21:23] for a in seen}) == 1 and [a[14] for a in seen] == [0, 4, 0, 0]
