@@ -939,7 +939,8 @@ def fmha_decode_step(q, knew, vnew, k_cache, v_cache, seqlen_k, block_table, *, 
 
 def shared_prefix_splits(batch, num_groups, max_group_size, q_num_heads, kv_num_heads, seqlen_q, head_dim, max_prefix_len,
                          max_own_len, num_cu=0) -> Tuple[int, int]:
-    """(prefix splits, own splits) fmha_decode_shared_prefix takes by default, from the CU count and the key counts."""
+    """(prefix splits, own splits) from the CU count, the longest prefix and the most keys behind one.  By default
+    fmha_decode_shared_prefix takes these, and more own splits where a sequence without the longest prefix may need them."""
     ns = (ctypes.c_int32(), ctypes.c_int32())
     _call("fck_fmha_shared_prefix_splits", batch, num_groups, max_group_size, q_num_heads, kv_num_heads, seqlen_q, head_dim,
           max_prefix_len, max_own_len, num_cu, ctypes.byref(ns[0]), ctypes.byref(ns[1]))
