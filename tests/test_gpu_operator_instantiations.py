@@ -47,7 +47,7 @@ def _shared(fmha, seed, sizes, prefixes, own, sq, hq, hk, d, dtype, page, flags)
     if fp8:
         kw.update(k_descale=0.5, v_descale=0.25)
     o = fmha.fmha_decode_shared_prefix(dev(q), dev(kc), dev(vc), _i32(lens), dev(table), _i32(prefixes), cu_groups=_i32(starts), lse=lse,
-                                       num_prefix_splits=2, num_splits=2, logits_soft_cap=cap, **kw).cpu()
+                                       num_prefix_splits=2, num_splits=2, max_group_size=max(sizes), logits_soft_cap=cap, **kw).cpu()
     assert torch.isfinite(o.float()).all()
     assert (o.double() - ref).abs().max() <= (2 * U[dtype] + 2.0 ** -20) * 6.0
     assert torch.equal(torch.isinf(lse.cpu()), torch.isinf(ref_lse))
